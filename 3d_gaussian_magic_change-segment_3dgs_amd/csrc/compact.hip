@@ -1,0 +1,726 @@
+// compact.hip -- the compact-scene kernels of include/gsr_compact.h: 4-bit microscaled
+// rows, colours from them with their gradients, eviction of the lightest Gaussians.
+#include "gsr_internal.h"
+#include "../../include/gsr_compact.h"
+
+namespace gsr {
+namespace {
+
+constexpr int CP_THREADS = 256;
+
+int launched(const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return set_error(std::string("[gsr] ") + what + ": " + hipGetErrorString(e));
+    return 0;
+}
+
+__host__ __device__ inline int mx_words(int K) { return (K + 7) / 8; }
+__host__ __device__ inline int mx_blocks(int K) { return (K + GSR_MX_BLOCK - 1) / GSR_MX_BLOCK; }
+
+// ------------------------------------------------------------------ 4-bit rows --
+// The gfx950 converts do the whole of the rounding: v_cvt_scalef32_pk_fp4_f32 divides by
+// 2^(exponent field - 127) and rounds to E2M1 (nearest, ties to even, saturating; exponent
+// field 0 is 2^-127, 255 is NaN when read back), so the scale byte goes in as the bits of a float.
+typedef float f2v __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float mx_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+__device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], float scale) {
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
+    return w;
+}
+
+__device__ __forceinline__ void mx_decode8(uint32_t w, float scale, float* v) {
+    const f2v a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0);
+    const f2v b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1);
+    const f2v c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2);
+    const f2v d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3);
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+    v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+}
+
+// Scale byte of a block from the largest |x| as bits (an unsigned maximum: NaN and infinity
+// come out on top).  floor(log2) - 2 is the exponent field less two, from 0 upwards.
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
+    const uint32_t e = amax_bits >> 23;
+    return e == 255u ? 255u : (e > 2u ? e : 2u) - 2u;
+}
+
+// Four lanes per block, eight values (one code word) each; the four share the maximum.
+__global__ void __launch_bounds__(CP_THREADS) k_mx4_quantize(long long R, int K, const float* __restrict__ x,
+                                                             long long stride, uint32_t* __restrict__ codes,
+                                                             uint8_t* __restrict__ scales) {
+    const int nb = mx_blocks(K), nw = mx_words(K);
+    const long long total = R * nb * 4;
+    const int sub = threadIdx.x & 3;
+    for (long long t = (long long)blockIdx.x * CP_THREADS + threadIdx.x; t < total;
+         t += (long long)gridDim.x * CP_THREADS) {  // whole quads stay together: total % 4 == 0
+        const long long q = t >> 2;
+        const long long row = q / nb;
+        const int b = (int)(q - row * nb);
+        const int k0 = b * GSR_MX_BLOCK + sub * 8;
+        const float* p = x + row * stride + k0;
+        float v[8];
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = k0 + j < K ? p[j] : 0.0f;
+            const uint32_t a = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+            m = m > a ? m : a;
+        }
+        uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true);  // quad_perm 1 0 3 2
+        m = m > o ? m : o;
+        o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true);  // quad_perm 2 3 0 1
+        m = m > o ? m : o;
+        const uint32_t s = mx_scale_byte(m);
+        if (k0 < K) codes[row * nw + b * 4 + sub] = s == 255u ? 0u : mx_encode8(v, mx_scale(s));
+        if (sub == 0) scales[row * nb + b] = (uint8_t)s;
+    }
+}
+
+__global__ void __launch_bounds__(CP_THREADS) k_mx4_dequantize(long long R, int K, const uint32_t* __restrict__ codes,
+                                                               const uint8_t* __restrict__ scales,
+                                                               float* __restrict__ x) {
+    const int nb = mx_blocks(K), nw = mx_words(K);
+    const long long total = R * nw;
+    for (long long t = (long long)blockIdx.x * CP_THREADS + threadIdx.x; t < total;
+         t += (long long)gridDim.x * CP_THREADS) {
+        const long long row = t / nw;
+        const int w = (int)(t - row * nw);
+        float v[8];
+        mx_decode8(codes[t], mx_scale(scales[row * nb + (w >> 2)]), v);
+        float* p = x + row * K + w * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (w * 8 + j < K) p[j] = v[j];
+    }
+}
+
+// --------------------------------------------------------------------- colours --
+// Real spherical harmonics up to degree 3 in the reference's order and signs
+// (utils/sh_utils.py:26-48); F = float, or double where a sign needs it.
+template <int DEG, typename F>
+__device__ __forceinline__ void sh_values(F x, F y, F z, F* b) {
+    b[0] = (F)0.28209479177387814;
+    if constexpr (DEG > 0) {
+        const F c1 = (F)0.4886025119029199;
+        b[1] = -c1 * y; b[2] = c1 * z; b[3] = -c1 * x;
+    }
+    if constexpr (DEG > 1) {
+        const F a = (F)1.0925484305920792, c = (F)0.31539156525252005, e = (F)0.5462742152960396;
+        const F xx = x * x, yy = y * y, zz = z * z;
+        b[4] = a * (x * y); b[5] = -a * (y * z); b[6] = c * ((F)2 * zz - xx - yy); b[7] = -a * (x * z);
+        b[8] = e * (xx - yy);
+        if constexpr (DEG > 2) {
+            const F p = (F)0.5900435899266435, q = (F)2.890611442640554, r = (F)0.4570457994644658,
+                    s = (F)0.3731763325901154, u = (F)1.445305721320277;
+            b[9] = -p * y * ((F)3 * xx - yy);
+            b[10] = q * (x * y) * z;
+            b[11] = -r * y * ((F)4 * zz - xx - yy);
+            b[12] = s * z * ((F)2 * zz - (F)3 * xx - (F)3 * yy);
+            b[13] = -r * x * ((F)4 * zz - xx - yy);
+            b[14] = u * z * (xx - yy);
+            b[15] = -p * x * (xx - (F)3 * yy);
+        }
+    }
+}
+
+// sum_k w[k] grad Y_k at (x, y, z) (gradients of the polynomials above; what they have along
+// (x, y, z) itself drops out in the projection that follows).
+template <int DEG>
+__device__ __forceinline__ void sh_grad(float x, float y, float z, const float* w, float& gx, float& gy, float& gz) {
+    gx = gy = gz = 0.0f;
+    if constexpr (DEG > 0) {
+        const float c1 = 0.4886025119029199f;
+        gx = -c1 * w[3]; gy = -c1 * w[1]; gz = c1 * w[2];
+    }
+    if constexpr (DEG > 1) {
+        const float a = 1.0925484305920792f, c = 0.31539156525252005f, e = 0.5462742152960396f;
+        gx += a * (y * w[4] - z * w[7]) - 2.0f * c * x * w[6] + 2.0f * e * x * w[8];
+        gy += a * (x * w[4] - z * w[5]) - 2.0f * c * y * w[6] - 2.0f * e * y * w[8];
+        gz += -a * (y * w[5] + x * w[7]) + 4.0f * c * z * w[6];
+        if constexpr (DEG > 2) {
+            const float p = 0.5900435899266435f, q = 2.890611442640554f, r = 0.4570457994644658f,
+                        s = 0.3731763325901154f, u = 1.445305721320277f;
+            const float xx = x * x, yy = y * y, zz = z * z, xy = x * y, yz = y * z, xz = x * z;
+            gx += -6.0f * p * xy * w[9] + q * yz * w[10] + 2.0f * r * xy * w[11] - 6.0f * s * xz * w[12] -
+                  r * (4.0f * zz - 3.0f * xx - yy) * w[13] + 2.0f * u * xz * w[14] - 3.0f * p * (xx - yy) * w[15];
+            gy += -3.0f * p * (xx - yy) * w[9] + q * xz * w[10] - r * (4.0f * zz - xx - 3.0f * yy) * w[11] -
+                  6.0f * s * yz * w[12] + 2.0f * r * xy * w[13] - 2.0f * u * yz * w[14] + 6.0f * p * xy * w[15];
+            gz += q * xy * w[10] - 8.0f * r * yz * w[11] + 3.0f * s * (2.0f * zz - xx - yy) * w[12] -
+                  8.0f * r * xz * w[13] + u * (xx - yy) * w[14];
+        }
+    }
+}
+
+// Decoded coefficients of one Gaussian, 3 floats each, coefficient 0 the constant one.
+template <int DEG>
+struct Coef {
+    static constexpr int N = (DEG + 1) * (DEG + 1);
+    static constexpr int WORDS = (3 * (N - 1) + 7) / 8;
+    float q[8 * WORDS + 3];
+    __device__ __forceinline__ void load(int i, int pitch, int nb, const float* __restrict__ dc, long long dc_stride,
+                                         const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales) {
+        const float* d = dc + i * dc_stride;
+        q[0] = d[0]; q[1] = d[1]; q[2] = d[2];
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w)
+            mx_decode8(codes[(long long)i * pitch + w], mx_scale(scales[(long long)i * nb + (w >> 2)]), q + 3 + 8 * w);
+    }
+};
+
+struct ShArgs {
+    int P, V, pitch, nb, M;
+    const float* xyz;
+    const float* dc;
+    long long dc_stride;
+    const uint32_t* codes;
+    const uint8_t* scales;
+    const float* campos;
+};
+
+// u -> u / |u|; returns 1 / |u|, 0 (and d = 0) where u is 0.
+__device__ __forceinline__ float normalize3(float& x, float& y, float& z) {
+    float n = x * x + y * y + z * z, m = 1.0f;
+    if (!(n > 1e-30f && n < 1e30f)) {  // the squares leave the range (or u is 0, or not finite)
+        m = fmaxf(fabsf(x), fmaxf(fabsf(y), fabsf(z)));
+        if (!(m > 0.0f)) return 0.0f;
+        x /= m; y /= m; z /= m;
+        n = x * x + y * y + z * z;
+    }
+    const float r = 1.0f / sqrtf(n);
+    x *= r; y *= r; z *= r;
+    return r / m;
+}
+
+template <int DEG>
+__global__ void __launch_bounds__(CP_THREADS) k_sh_colors(ShArgs a, float* __restrict__ colors) {
+    const int i = blockIdx.x * CP_THREADS + threadIdx.x;
+    if (i >= a.P) return;
+    Coef<DEG> c;
+    c.load(i, a.pitch, a.nb, a.dc, a.dc_stride, a.codes, a.scales);
+    const float px = a.xyz[3LL * i], py = a.xyz[3LL * i + 1], pz = a.xyz[3LL * i + 2];
+    for (int v = 0; v < a.V; ++v) {
+        float x = px - a.campos[3 * v], y = py - a.campos[3 * v + 1], z = pz - a.campos[3 * v + 2];
+        normalize3(x, y, z);
+        float b[Coef<DEG>::N];
+        sh_values<DEG, float>(x, y, z, b);
+        float s[3] = {0.5f, 0.5f, 0.5f};
+#pragma unroll
+        for (int k = 0; k < Coef<DEG>::N; ++k)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) s[j] += b[k] * c.q[3 * k + j];
+        float* o = colors + ((long long)v * a.P + i) * 3;
+#pragma unroll
+        for (int j = 0; j < 3; ++j) o[j] = s[j] < 0.0f ? 0.0f : s[j];  // keeps a NaN
+    }
+}
+
+// The value before the clamp in 64 bits.
+template <int DEG>
+__device__ void preclamp64(const Coef<DEG>& c, float px, float py, float pz, const float* cam, double* s) {
+    const double x = (double)px - cam[0], y = (double)py - cam[1], z = (double)pz - cam[2];
+    const double n = x * x + y * y + z * z;
+    const double r = n > 0.0 ? 1.0 / sqrt(n) : 0.0;
+    double b[Coef<DEG>::N];
+    sh_values<DEG, double>(x * r, y * r, z * r, b);
+    s[0] = s[1] = s[2] = 0.5;
+#pragma unroll
+    for (int k = 0; k < Coef<DEG>::N; ++k)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) s[j] += b[k] * (double)c.q[3 * k + j];
+}
+
+template <int DEG>
+__global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, const float* __restrict__ dcolors,
+                                                                   float* __restrict__ dxyz, float* __restrict__ ddc,
+                                                                   float* __restrict__ dfeatures) {
+    constexpr int N = Coef<DEG>::N;
+    const int i = blockIdx.x * CP_THREADS + threadIdx.x;
+    if (i >= a.P) return;
+    Coef<DEG> c;
+    c.load(i, a.pitch, a.nb, a.dc, a.dc_stride, a.codes, a.scales);
+    const float px = a.xyz[3LL * i], py = a.xyz[3LL * i + 1], pz = a.xyz[3LL * i + 2];
+    // Rounding of the value before the clamp: a direction is good to 3 ulp of 1, a basis value
+    // (slope at most 4) to 32, so a channel's sum to 2^-19 of its coefficients' sum; inside twice
+    // that the sign is taken from 64 bits.
+    float near[3] = {0.5f, 0.5f, 0.5f};
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) near[j] += fabsf(c.q[3 * k + j]);
+#pragma unroll
+    for (int j = 0; j < 3; ++j) near[j] *= 0x1p-18f;
+    float acc[3 * N];
+#pragma unroll
+    for (int k = 0; k < 3 * N; ++k) acc[k] = 0.0f;
+    float ax = 0.0f, ay = 0.0f, az = 0.0f;
+    for (int v = 0; v < a.V; ++v) {
+        const float* cam = a.campos + 3 * v;
+        float x = px - cam[0], y = py - cam[1], z = pz - cam[2];
+        const float r = normalize3(x, y, z);
+        float b[N], s[3] = {0.5f, 0.5f, 0.5f};
+        sh_values<DEG, float>(x, y, z, b);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) s[j] += b[k] * c.q[3 * k + j];
+        bool on[3];
+        bool close = false;
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            on[j] = s[j] >= 0.0f;
+            close |= fabsf(s[j]) < near[j];
+        }
+        if (close) {
+            double t[3];
+            preclamp64<DEG>(c, px, py, pz, cam, t);
+#pragma unroll
+            for (int j = 0; j < 3; ++j) on[j] = t[j] >= 0.0;
+        }
+        const float* gp = dcolors + ((long long)v * a.P + i) * 3;
+        float g[3];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) g[j] = on[j] ? gp[j] : 0.0f;
+        float w[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            w[k] = c.q[3 * k] * g[0] + c.q[3 * k + 1] * g[1] + c.q[3 * k + 2] * g[2];
+#pragma unroll
+            for (int j = 0; j < 3; ++j) acc[3 * k + j] += b[k] * g[j];
+        }
+        float gx, gy, gz;
+        sh_grad<DEG>(x, y, z, w, gx, gy, gz);
+        const float along = gx * x + gy * y + gz * z;
+        ax += r * (gx - along * x);
+        ay += r * (gy - along * y);
+        az += r * (gz - along * z);
+    }
+    if (dxyz) {
+        dxyz[3LL * i] = ax; dxyz[3LL * i + 1] = ay; dxyz[3LL * i + 2] = az;
+    }
+    if (ddc)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) ddc[3LL * i + j] = acc[j];
+    if (dfeatures) {
+        float* o = dfeatures + 3LL * a.M * i;
+#pragma unroll
+        for (int k = 0; k < 3 * N; ++k) o[k] = acc[k];
+        for (int k = 3 * N; k < 3 * a.M; ++k) o[k] = 0.0f;
+    }
+}
+
+__global__ void __launch_bounds__(CP_THREADS) k_accumulate_weights(int P, const float* __restrict__ w,
+                                                                   long long stride, float decay,
+                                                                   float* __restrict__ acc) {
+    const int i = blockIdx.x * CP_THREADS + threadIdx.x;
+    if (i < P) acc[i] = decay * acc[i] + w[i * stride];
+}
+
+// -------------------------------------------------------------------- eviction --
+// The rows to keep of a group are its last `recent` ones and the heaviest `pick` of those
+// before them.  Radix selection: three histogram passes (11, 11, 10 bits from the top) find the
+// key T of the pick-th heaviest row and how many of the rows equal to it are kept (`ties`, the
+// lowest first); a count and a write pass then put the ids in order.  Every count is an
+// integer, so the result does not depend on the order of the atomics.
+constexpr int KEEP_TILE = CP_THREADS * 16;  // rows per block
+constexpr int KEEP_BINS = 2048;
+
+struct KeepGroup {
+    int begin, end, old_end;  // rows [begin, old_end) compete, [old_end, end) are kept
+    int pick;
+    int out;    // first output slot
+    int tile0;  // first tile
+};
+struct KeepArgs {
+    int n, tiles;
+    KeepGroup g[GSR_KEEP_MAX_GROUPS];
+};
+struct KeepSel {
+    uint32_t prefix, need;  // digits found so far; the rank looked for among the keys that share them
+};
+struct KeepWs {
+    uint32_t* hist;  // [groups][3][KEEP_BINS]
+    KeepSel* sel;    // [groups][3]
+    uint2* count;    // [tiles] rows above T, rows equal to T
+};
+inline size_t keep_tiles(size_t P) { return P / KEEP_TILE + GSR_KEEP_MAX_GROUPS + 1; }
+inline size_t keep_hist_bytes() { return (size_t)GSR_KEEP_MAX_GROUPS * 3 * KEEP_BINS * 4; }
+inline KeepWs keep_ws(void* p) {
+    char* c = static_cast<char*>(p);
+    KeepWs w;
+    w.hist = reinterpret_cast<uint32_t*>(c);
+    w.sel = reinterpret_cast<KeepSel*>(c + keep_hist_bytes());
+    w.count = reinterpret_cast<uint2*>(c + keep_hist_bytes() + align_up(GSR_KEEP_MAX_GROUPS * 3 * sizeof(KeepSel)));
+    return w;
+}
+
+// Weights in the order of unsigned integers: NaN lowest, -0 as +0.
+__device__ __forceinline__ uint32_t keep_key(float w) {
+    if (w != w) return 0u;
+    const uint32_t u = w == 0.0f ? 0u : __float_as_uint(w);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ int keep_group_of(const KeepArgs& a, int tile) {
+    int lo = 0, hi = a.n - 1;
+    while (lo < hi) {
+        const int m = (lo + hi + 1) >> 1;
+        if (a.g[m].tile0 <= tile) lo = m;
+        else hi = m - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive, DPP row shifts and broadcasts
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
+    return x;
+}
+
+// Exclusive scan over the block's threads; every thread calls it.
+template <int THREADS>
+__device__ __forceinline__ uint32_t block_scan_excl(uint32_t x, uint32_t* s_wave) {
+    const uint32_t inc = wave_scan(x);
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) s_wave[wave] = inc;
+    __syncthreads();
+    uint32_t base = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) base += w < wave ? s_wave[w] : 0u;
+    return base + inc - x;
+}
+
+// The bin, counted from the top, that holds the need-th largest key, and the rank inside it
+// (need >= 1 and at most the sum of the bins).
+template <int THREADS>
+__device__ __forceinline__ KeepSel find_bin(const uint32_t* hist, uint32_t need, uint32_t* s_wave, KeepSel* s_out) {
+    constexpr int PER = KEEP_BINS / THREADS;
+    const int top = KEEP_BINS - 1 - (int)threadIdx.x * PER;
+    uint32_t h[PER], sum = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) sum += h[k] = hist[top - k];
+    uint32_t above = block_scan_excl<THREADS>(sum, s_wave);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        if (above < need && need <= above + h[k]) *s_out = {(uint32_t)(top - k), need - above};
+        above += h[k];
+    }
+    __syncthreads();
+    return *s_out;
+}
+
+__global__ void __launch_bounds__(CP_THREADS) k_keep_clear(uint32_t* __restrict__ p, int n) {
+    for (int i = blockIdx.x * CP_THREADS + threadIdx.x; i < n; i += gridDim.x * CP_THREADS) p[i] = 0u;
+}
+
+// Digits found before pass PASS of group g: the first tile's block leaves them for the later
+// kernels, every block works them out for itself.
+template <int PASS>
+__device__ __forceinline__ KeepSel keep_state(const KeepArgs& a, const KeepWs& ws, int g, int tile, uint32_t* s_wave,
+                                              KeepSel* s_out) {
+    KeepSel prev = {0u, (uint32_t)a.g[g].pick};
+    if constexpr (PASS == 0) return prev;
+    if (PASS > 1) prev = ws.sel[g * 3 + PASS - 2];
+    const KeepSel b = find_bin<CP_THREADS>(ws.hist + ((size_t)g * 3 + PASS - 1) * KEEP_BINS, prev.need, s_wave, s_out);
+    const KeepSel now = {(prev.prefix << (PASS == 3 ? 10 : 11)) | b.prefix, b.need};
+    if (tile == a.g[g].tile0 && threadIdx.x == 0) ws.sel[g * 3 + PASS - 1] = now;
+    return now;
+}
+
+template <int PASS>
+__global__ void __launch_bounds__(CP_THREADS) k_keep_hist(KeepArgs a, KeepWs ws, const float* __restrict__ w) {
+    __shared__ uint32_t h[KEEP_BINS];
+    __shared__ uint32_t s_wave[CP_THREADS / 64];
+    __shared__ KeepSel s_out;
+    const int tile = blockIdx.x, g = keep_group_of(a, tile);
+    const KeepGroup G = a.g[g];
+    if (G.pick == 0) return;  // nothing to look for (the whole block)
+    for (int k = threadIdx.x; k < KEEP_BINS; k += CP_THREADS) h[k] = 0u;
+    const KeepSel st = keep_state<PASS>(a, ws, g, tile, s_wave, &s_out);
+    __syncthreads();
+    const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE;
+#pragma unroll 4
+    for (int k = 0; k < 16; ++k) {
+        const long long i = base + k * CP_THREADS + threadIdx.x;
+        if (i < G.old_end) {
+            const uint32_t key = keep_key(w[i]);
+            const bool in = PASS == 0 || (PASS == 1 ? key >> 21 : key >> 10) == st.prefix;
+            const uint32_t d = PASS == 0 ? key >> 21 : PASS == 1 ? (key >> 10) & 2047u : key & 1023u;
+            if (in) atomicAdd(&h[d], 1u);
+        }
+    }
+    __syncthreads();
+    uint32_t* out = ws.hist + ((size_t)g * 3 + PASS) * KEEP_BINS;
+    for (int k = threadIdx.x; k < KEEP_BINS; k += CP_THREADS)
+        if (h[k]) atomicAdd(&out[k], h[k]);
+}
+
+// Rows above / equal to T in each tile.
+__global__ void __launch_bounds__(CP_THREADS) k_keep_count(KeepArgs a, KeepWs ws, const float* __restrict__ w) {
+    __shared__ uint32_t s_wave[CP_THREADS / 64];
+    __shared__ KeepSel s_out;
+    const int tile = blockIdx.x, g = keep_group_of(a, tile);
+    const KeepGroup G = a.g[g];
+    uint32_t gt = 0, eq = 0;
+    if (G.pick > 0) {
+        const uint32_t T = keep_state<3>(a, ws, g, tile, s_wave, &s_out).prefix;
+        const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE;
+        for (int k = 0; k < 16; ++k) {
+            const long long i = base + k * CP_THREADS + threadIdx.x;
+            if (i < G.old_end) {
+                const uint32_t key = keep_key(w[i]);
+                gt += key > T;
+                eq += key == T;
+            }
+        }
+    }
+    const uint32_t both = gt | eq << 16;  // at most KEEP_TILE = 4096 of each
+    const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave);
+    if (threadIdx.x == CP_THREADS - 1) ws.count[tile] = make_uint2((before + both) & 0xFFFFu, (before + both) >> 16);
+}
+
+// Thread t writes rows [16 t, 16 t + 16) of its tile: slot = first slot + kept rows before.
+__global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws, const float* __restrict__ w,
+                                                           int* __restrict__ ids) {
+    __shared__ uint32_t s_wave[CP_THREADS / 64];
+    __shared__ unsigned long long s_sum;
+    const int tile = blockIdx.x, g = keep_group_of(a, tile);
+    const KeepGroup G = a.g[g];
+    const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE + threadIdx.x * 16;
+    uint32_t T = 0xFFFFFFFFu, ties = 0;  // no key reaches this T
+    uint32_t gt0 = 0, eq0 = 0;
+    if (G.pick > 0) {
+        const KeepSel st = ws.sel[g * 3 + 2];
+        T = st.prefix;
+        ties = st.need;
+        if (threadIdx.x == 0) s_sum = 0;
+        __syncthreads();
+        unsigned long long sum = 0;
+        for (int t = G.tile0 + threadIdx.x; t < tile; t += CP_THREADS) {
+            const uint2 c = ws.count[t];
+            sum += c.x | (unsigned long long)c.y << 32;
+        }
+        if (sum) atomicAdd(&s_sum, sum);
+        __syncthreads();
+        gt0 = (uint32_t)s_sum;
+        eq0 = (uint32_t)(s_sum >> 32);
+    }
+    uint32_t key[16], both = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        key[k] = base + k < G.old_end ? keep_key(w[base + k]) : 0u;
+        const bool in = base + k < G.old_end;
+        both += (in && key[k] > T ? 1u : 0u) + (in && key[k] == T ? 1u << 16 : 0u);
+    }
+    const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave);
+    gt0 += before & 0xFFFFu;
+    eq0 += before >> 16;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const long long i = base + k;
+        if (i >= G.end) break;
+        if (i >= G.old_end) {
+            ids[G.out + G.pick + (i - G.old_end)] = (int)i;
+            continue;
+        }
+        const bool up = key[k] > T, tie = key[k] == T;
+        if (up || (tie && eq0 < ties)) ids[G.out + gt0 + (eq0 < ties ? eq0 : ties)] = (int)i;
+        gt0 += up;
+        eq0 += tie;
+    }
+}
+
+// ------------------------------------------------------------------------ rows --
+constexpr int TAKE_MAX = 32;
+struct TakeArgs {
+    gsr_rows t[TAKE_MAX];
+};
+__global__ void __launch_bounds__(CP_THREADS) k_take_rows(TakeArgs a, int K, const int* __restrict__ ids) {
+    const gsr_rows t = a.t[blockIdx.y];
+    const uint32_t* src = static_cast<const uint32_t*>(t.src);
+    uint32_t* dst = static_cast<uint32_t*>(t.dst);
+    const long long n = (long long)K * t.width;
+    for (long long e = (long long)blockIdx.x * CP_THREADS + threadIdx.x; e < n + t.pad;
+         e += (long long)gridDim.x * CP_THREADS) {
+        uint32_t v = 0;
+        if (e < n) {
+            const int row = (int)(e / t.width);
+            const int id = ids[row];
+            if ((unsigned)id < (unsigned)t.rows) v = src[(long long)id * t.width + (e - (long long)row * t.width)];
+        }
+        dst[e] = v;
+    }
+}
+
+unsigned grid_for(long long items, long long cap) {
+    const long long g = (items + CP_THREADS - 1) / CP_THREADS;
+    return (unsigned)(g < 1 ? 1 : g > cap ? cap : g);
+}
+
+int check_rows(long long R, int K) {
+    if (R < 0 || K < 0 || K > (1 << 20)) return set_error("[gsr] mx4: invalid number or width of rows");
+    return 0;
+}
+
+int check_colors(int P, int V, int degree, int M, const float* xyz, const float* dc, const uint32_t* codes,
+                 const uint8_t* scales, const float* campos) {
+    if (P < 0 || V < 1 || V > GSR_MAX_VIEWS) return set_error("[gsr] sh_colors: invalid P or number of views");
+    if (degree < 0 || degree > 3 || M < (degree + 1) * (degree + 1) || M > 16)
+        return set_error("[gsr] sh_colors: degree must be 0..3 with (degree + 1)^2 <= M <= 16");
+    if (P > 0 && (!xyz || !dc || !campos || (M > 1 && (!codes || !scales))))
+        return set_error("[gsr] sh_colors: null buffer");
+    return 0;
+}
+
+ShArgs sh_args(int P, int V, int M, const float* xyz, const float* dc, long long dc_stride, const uint32_t* codes,
+               const uint8_t* scales, const float* campos) {
+    return {P, V, mx_words(3 * (M - 1)), mx_blocks(3 * (M - 1)), M, xyz, dc, dc_stride, codes, scales, campos};
+}
+
+}  // namespace
+}  // namespace gsr
+
+using namespace gsr;
+
+extern "C" {
+
+GSR_API int gsr_mx4_quantize(long long R, int K, const float* x, long long row_stride, uint32_t* codes,
+                             uint8_t* scales, void* stream) {
+    if (int rc = check_rows(R, K)) return rc;
+    if (R == 0 || K == 0) return 0;
+    if (!x || !codes || !scales) return set_error("[gsr] gsr_mx4_quantize: null buffer");
+    if (row_stride < K && R > 1) return set_error("[gsr] gsr_mx4_quantize: rows overlap");
+    k_mx4_quantize<<<grid_for(R * mx_blocks(K) * 4, 1 << 20), CP_THREADS, 0, (hipStream_t)stream>>>(
+        R, K, x, row_stride, codes, scales);
+    return launched("mx4_quantize");
+}
+
+GSR_API int gsr_mx4_dequantize(long long R, int K, const uint32_t* codes, const uint8_t* scales, float* x,
+                               void* stream) {
+    if (int rc = check_rows(R, K)) return rc;
+    if (R == 0 || K == 0) return 0;
+    if (!x || !codes || !scales) return set_error("[gsr] gsr_mx4_dequantize: null buffer");
+    k_mx4_dequantize<<<grid_for(R * mx_words(K), 1 << 20), CP_THREADS, 0, (hipStream_t)stream>>>(R, K, codes, scales,
+                                                                                              x);
+    return launched("mx4_dequantize");
+}
+
+GSR_API int gsr_sh_colors(int P, int V, int degree, int M, const float* xyz, const float* dc, long long dc_stride,
+                          const uint32_t* codes, const uint8_t* scales, const float* campos, float* colors,
+                          void* stream) {
+    if (int rc = check_colors(P, V, degree, M, xyz, dc, codes, scales, campos)) return rc;
+    if (P == 0) return 0;
+    if (!colors) return set_error("[gsr] gsr_sh_colors: null buffer");
+    const ShArgs a = sh_args(P, V, M, xyz, dc, dc_stride, codes, scales, campos);
+    const unsigned grid = grid_for(P, 1LL << 31);
+    hipStream_t st = (hipStream_t)stream;
+    if (degree == 0) k_sh_colors<0><<<grid, CP_THREADS, 0, st>>>(a, colors);
+    else if (degree == 1) k_sh_colors<1><<<grid, CP_THREADS, 0, st>>>(a, colors);
+    else if (degree == 2) k_sh_colors<2><<<grid, CP_THREADS, 0, st>>>(a, colors);
+    else k_sh_colors<3><<<grid, CP_THREADS, 0, st>>>(a, colors);
+    return launched("sh_colors");
+}
+
+GSR_API int gsr_sh_colors_backward(int P, int V, int degree, int M, const float* xyz, const float* dc,
+                                   long long dc_stride, const uint32_t* codes, const uint8_t* scales,
+                                   const float* campos, const float* dcolors, float* dxyz, float* ddc,
+                                   float* dfeatures, void* stream) {
+    if (int rc = check_colors(P, V, degree, M, xyz, dc, codes, scales, campos)) return rc;
+    if (P == 0 || (!dxyz && !ddc && !dfeatures)) return 0;
+    if (!dcolors) return set_error("[gsr] gsr_sh_colors_backward: null buffer");
+    const ShArgs a = sh_args(P, V, M, xyz, dc, dc_stride, codes, scales, campos);
+    const unsigned grid = grid_for(P, 1LL << 31);
+    hipStream_t st = (hipStream_t)stream;
+    if (degree == 0) k_sh_colors_backward<0><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures);
+    else if (degree == 1) k_sh_colors_backward<1><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures);
+    else if (degree == 2) k_sh_colors_backward<2><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures);
+    else k_sh_colors_backward<3><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures);
+    return launched("sh_colors_backward");
+}
+
+GSR_API int gsr_accumulate_weights(int P, const float* weights, long long stride, float decay, float* acc,
+                                   void* stream) {
+    if (P < 0) return set_error("[gsr] gsr_accumulate_weights: P < 0");
+    if (P == 0) return 0;
+    if (!weights || !acc) return set_error("[gsr] gsr_accumulate_weights: null buffer");
+    k_accumulate_weights<<<grid_for(P, 1LL << 31), CP_THREADS, 0, (hipStream_t)stream>>>(P, weights, stride, decay, acc);
+    return launched("accumulate_weights");
+}
+
+GSR_API size_t gsr_keep_ws_bytes(int P) {
+    return keep_hist_bytes() + align_up(GSR_KEEP_MAX_GROUPS * 3 * sizeof(KeepSel)) +
+           align_up(keep_tiles(P > 0 ? (size_t)P : 0) * sizeof(uint2));
+}
+
+GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const gsr_keep_group* groups, int* ids,
+                              void* ws, void* stream) {
+    if (P < 0 || n_groups < 0 || n_groups > GSR_KEEP_MAX_GROUPS)
+        return set_error("[gsr] gsr_keep_heaviest: at most " + std::to_string(GSR_KEEP_MAX_GROUPS) + " groups a call");
+    if (n_groups > 0 && !groups) return set_error("[gsr] gsr_keep_heaviest: null groups");
+    KeepArgs a{};
+    int last = 0;
+    long long out = 0;
+    for (int g = 0; g < n_groups; ++g) {
+        const gsr_keep_group& q = groups[g];
+        if (q.begin < last || q.end < q.begin || q.end > P)
+            return set_error("[gsr] gsr_keep_heaviest: groups must be ascending ranges of rows that do not overlap");
+        if (q.keep < 0 || q.keep > q.end - q.begin || q.recent < 0 || q.recent > q.keep)
+            return set_error("[gsr] gsr_keep_heaviest: 0 <= recent <= keep <= rows of the group");
+        last = q.end;
+        if (q.keep == 0) continue;  // nothing to write
+        a.g[a.n++] = {q.begin, q.end, q.end - q.recent, q.keep - q.recent, (int)out, a.tiles};
+        a.tiles += (q.end - q.begin + KEEP_TILE - 1) / KEEP_TILE;
+        out += q.keep;
+    }
+    if (a.n == 0) return 0;
+    if (!weights || !ids || !ws) return set_error("[gsr] gsr_keep_heaviest: null buffer");
+    hipStream_t st = (hipStream_t)stream;
+    const KeepWs w = keep_ws(ws);
+    const int words = a.n * 3 * KEEP_BINS;
+    k_keep_clear<<<grid_for(words, 1024), CP_THREADS, 0, st>>>(w.hist, words);
+    k_keep_hist<0><<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);
+    k_keep_hist<1><<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);
+    k_keep_hist<2><<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);
+    k_keep_count<<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);
+    k_keep_write<<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights, ids);
+    return launched("keep_heaviest");
+}
+
+GSR_API int gsr_take_rows(int K, const int* ids, int n, const gsr_rows* tensors, void* stream) {
+    if (K < 0 || n < 0 || (n > 0 && !tensors) || (K > 0 && n > 0 && !ids))
+        return set_error("[gsr] gsr_take_rows: invalid arguments");
+    for (int k = 0; k < n; ++k) {
+        const gsr_rows& t = tensors[k];
+        if (t.width < 0 || t.rows < 0 || t.pad < 0) return set_error("[gsr] gsr_take_rows: invalid width or rows");
+        const long long words = (long long)K * t.width;
+        if ((words > 0 && t.rows > 0 && !t.src) || (words + t.pad > 0 && !t.dst))
+            return set_error("[gsr] gsr_take_rows: null buffer");
+    }
+    hipStream_t st = (hipStream_t)stream;
+    bool any = false;
+    for (int k0 = 0; k0 < n; k0 += TAKE_MAX) {
+        TakeArgs a{};
+        const int m = n - k0 < TAKE_MAX ? n - k0 : TAKE_MAX;
+        long long most = 0;
+        for (int k = 0; k < m; ++k) {
+            a.t[k] = tensors[k0 + k];
+            most = std::max(most, (long long)K * a.t[k].width + a.t[k].pad);
+        }
+        if (most == 0) continue;
+        any = true;
+        k_take_rows<<<dim3(grid_for(most, 1 << 16), m), CP_THREADS, 0, st>>>(a, K, ids);
+    }
+    return any ? launched("take_rows") : 0;
+}
+
+}  // extern "C"

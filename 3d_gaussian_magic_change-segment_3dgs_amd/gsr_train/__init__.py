@@ -7,3 +7,5 @@ from .gaussian_model import GaussianModel, get_expon_lr_func, inverse_sigmoid, b
 from .optim import GaussianAdam  # noqa: F401
 from ._C import ArenaSpec  # noqa: F401
 from .knn import distCUDA2  # noqa: F401
+from .compact import (CompactGaussians, MX4Rows, accumulate_weights, keep_heaviest, mx4_quantize,  # noqa: F401
+                      sh_colors, sh_colors_quantized, take_rows)

@@ -27,6 +27,7 @@ import torch
 import torch.nn as nn
 
 from . import _C
+from . import compact as _compact
 from . import ply as _ply
 from .optim import GaussianAdam
 
@@ -112,6 +113,7 @@ class GaussianModel:
         self.optimizer = None
         self.percent_dense = 0
         self.spatial_lr_scale = 0
+        self.feature_bits = 32  # 4: get_colors rounds the SH coefficients as compact() stores them
         self._allocate(0)
 
     # ---- storage ------------------------------------------------------------------------
@@ -127,6 +129,7 @@ class GaussianModel:
         self.max_radii2D = torch.zeros(P, **f32)
         self.xyz_gradient_accum = torch.zeros((P, 1), **f32)
         self.denom = torch.zeros((P, 1), **f32)
+        self.contribution = torch.zeros((P, 1), **f32)  # accumulated blend weights (evict)
         self._params_changed()
 
     def _params_changed(self, act_fresh=False):
@@ -187,6 +190,13 @@ class GaussianModel:
         cov = L @ L.transpose(1, 2)
         idx = torch.tensor([[0, 0], [0, 1], [0, 2], [1, 1], [1, 2], [2, 2]], device=cov.device)
         return cov[:, idx[:, 0], idx[:, 1]]
+
+    def get_colors(self, campos):
+        """Colours seen from campos ([3] -> [P, 3], [V, 3] -> [V, P, 3]), for the rasterizer's
+        colors_precomp, with the SH coefficients above the constant one rounded to 4 bits
+        (their gradient goes straight through the rounding): training with feature_bits = 4
+        fits the scene that compact() will store."""
+        return _compact.sh_colors_quantized(self.get_xyz, self.get_features, campos, self.active_sh_degree)
 
     def oneupSHdegree(self):
         if self.active_sh_degree < self.max_sh_degree:
@@ -337,6 +347,7 @@ class GaussianModel:
         if opt is not None:
             opt._resize(m1n, m2n)
         P = spec.P
+        self.contribution = torch.zeros((P, 1), dtype=torch.float32, device=self.device)
         # densification_postfix (:402-404) resets the statistics; prune keeps the zeros
         self.xyz_gradient_accum = torch.zeros((P, 1), dtype=torch.float32, device=self.device)
         self.denom = torch.zeros((P, 1), dtype=torch.float32, device=self.device)
@@ -367,7 +378,7 @@ class GaussianModel:
     def prune_points(self, mask):
         """gaussian_model.py:340-357: drop mask[i] (bool [P]); moments and statistics
         follow the kept Gaussians (statistics are kept, not reset, like the reference)."""
-        keep_stats = (self.xyz_gradient_accum, self.denom, self.max_radii2D)
+        keep_stats = (self.xyz_gradient_accum, self.denom, self.max_radii2D, self.contribution)
         a = self._densify_args(_C.PRUNE_MASK)
         m = mask.reshape(-1).to(self.device, torch.bool).contiguous()
         counts = self._rebuild(a, mask=m)
@@ -375,7 +386,53 @@ class GaussianModel:
         self.xyz_gradient_accum = keep_stats[0][keep].contiguous()
         self.denom = keep_stats[1][keep].contiguous()
         self.max_radii2D = keep_stats[2][keep].contiguous()
+        self.contribution = keep_stats[3][keep].contiguous()
         return counts
+
+    # ---- eviction to a budget, 4-bit scenes (gsr_train.compact) -------------------------
+    @torch.no_grad()
+    def add_contribution_stats(self, weights, decay=1.0):
+        """contribution <- decay * contribution + weights: the blend weights alpha * T of every
+        Gaussian summed over a view's pixels (gsr_tools.train_demo.blend_weights), float32 [P]."""
+        _compact.accumulate_weights(self.contribution, weights, decay)
+
+    @torch.no_grad()
+    def evict(self, budget, recent=0, groups=None):
+        """Bring the model -- or, with groups = [(begin, end)] as merge_ply returns them, each of
+        its scenes -- to at most `budget` Gaussians (a number, or a list with one for each
+        group): the last `recent` ones (new Gaussians are appended) and the heaviest of the others by
+        `contribution` stay, in order, with their moments and statistics; Gaussians in no group
+        go.  The host does not wait for the device.  Returns (ids, groups): the old index of each
+        Gaussian (int32 [P]) and the groups' new ranges."""
+        plan = _compact._keep_groups("evict", self.num_points, budget, groups, recent)
+        ids = _compact.keep_heaviest(self.contribution, budget, groups, recent)
+        opt = self.optimizer
+        arenas = [self._arena.data] + ([opt.exp_avg, opt.exp_avg_sq] if opt is not None else [])
+        spec, new = _compact.take_gaussians(self._spec, ids, arenas)
+        stats = _compact.take_rows(ids, [self.xyz_gradient_accum, self.denom, self.max_radii2D, self.contribution])
+        self._spec = spec
+        self._arena = nn.Parameter(new[0])
+        self._act = torch.zeros(spec.act_total, dtype=torch.float32, device=self.device)
+        self._params_changed()
+        if opt is not None:
+            opt._resize(new[1], new[2])
+        self.xyz_gradient_accum, self.denom, self.max_radii2D, self.contribution = stats
+        ranges, o = [], 0
+        for _, _, k, _ in plan:
+            ranges.append((o, o + k))
+            o += k
+        return ids, ranges
+
+    @torch.no_grad()
+    def compact(self):
+        """The scene as it is rendered, with the SH coefficients above the constant one in 4
+        bits and no training state (CompactGaussians)."""
+        P = self.num_points
+        features = self.get_features
+        return _compact.CompactGaussians(
+            self.get_xyz.clone(), features[:, :1].clone(), _compact.mx4_quantize(features.view(P, -1)[:, 3:]),
+            self.get_opacity.clone(), self.get_scaling.clone(), self.get_rotation.clone(), self.get_segment.clone(),
+            self.active_sh_degree)
 
     def construct_list_of_attributes(self):
         """gaussian_model.py:187-205: PLY vertex property names in file order."""
