@@ -17,6 +17,34 @@ int launched(const char* what) {
 __host__ __device__ inline int mx_words(int K) { return (K + 7) / 8; }
 __host__ __device__ inline int mx_blocks(int K) { return (K + GSR_MX_BLOCK - 1) / GSR_MX_BLOCK; }
 
+// How the units of a row of a streamed tensor (R rows of `units`) go to blocks of `span`
+// lanes: whole rows where a row fits, so that no lane divides (units 12 of a 1024 span:
+// 85 rows, 99.6 % of the lanes); pieces of a row otherwise.
+struct Tiling {
+    int units, rows;  // rows a block (0: pieces)
+    uint32_t magic;   // 2^32 / units + 1: exact quotients of numbers below 2^32 / units
+};
+inline Tiling tiling(int units, int span) {
+    return {units, units <= span ? span / units : 0, units > 1 ? (uint32_t)((1ULL << 32) / units + 1) : 0u};
+}
+inline long long tiling_blocks(const Tiling& t, long long R, int span) {
+    return t.rows > 0 ? (R + t.rows - 1) / t.rows : (R * t.units + span - 1) / span;
+}
+template <int SPAN>
+__device__ __forceinline__ bool tiling_place(const Tiling& t, uint32_t block, uint32_t local, long long R,
+                                             long long& row, int& unit) {
+    if (t.rows > 0) {
+        const uint32_t r = t.units == 1 ? local : __umulhi(local, t.magic);
+        row = (long long)block * t.rows + r;
+        unit = (int)(local - r * t.units);
+        return r < (uint32_t)t.rows && row < R;
+    }
+    const long long e = (long long)block * SPAN + local;
+    row = e / t.units;
+    unit = (int)(e - row * t.units);
+    return row < R;
+}
+
 // ------------------------------------------------------------------ 4-bit rows --
 // The gfx950 converts do the whole of the rounding: v_cvt_scalef32_pk_fp4_f32 divides by
 // 2^(exponent field - 127) and rounds to E2M1 (nearest, ties to even, saturating; exponent
@@ -25,12 +53,14 @@ typedef float f2v __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float mx_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-__device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], float scale) {
+typedef float v4a __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes at any word
+
+__device__ __forceinline__ uint32_t mx_encode8(v4a lo, v4a hi, float scale) {
     uint32_t w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], scale, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, lo.x, lo.y, scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, lo.z, lo.w, scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, hi.x, hi.y, scale, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, hi.z, hi.w, scale, 3);
     return w;
 }
 
@@ -50,53 +80,81 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
     return e == 255u ? 255u : (e > 2u ? e : 2u) - 2u;
 }
 
-// Four lanes per block, eight values (one code word) each; the four share the maximum.
-__global__ void __launch_bounds__(CP_THREADS) k_mx4_quantize(long long R, int K, const float* __restrict__ x,
+
+// Values [k, k + 4) of a row of K, zeros behind its end.
+__device__ __forceinline__ v4a load4(const float* p, int k, int K) {
+    v4a r = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (k + 4 <= K) {
+        r = *reinterpret_cast<const v4a*>(p);
+    } else {
+        if (k < K) r.x = p[0];
+        if (k + 1 < K) r.y = p[1];
+        if (k + 2 < K) r.z = p[2];
+    }
+    return r;
+}
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, v4a v) {
+    const uint32_t x = __float_as_uint(v.x) & 0x7FFFFFFFu, y = __float_as_uint(v.y) & 0x7FFFFFFFu,
+                   z = __float_as_uint(v.z) & 0x7FFFFFFFu, w = __float_as_uint(v.w) & 0x7FFFFFFFu;
+    const uint32_t a = x > y ? x : y, b = z > w ? z : w, c = a > b ? a : b;
+    return m > c ? m : c;
+}
+
+// Four lanes per block, eight values (one code word) each; the four share the largest |x| through
+// DPP.  A thread takes MXQ_PER such pieces, their loads in flight together.
+constexpr int MXQ_PER = 2, MXQ_SPAN = CP_THREADS / 4 * MXQ_PER;
+__global__ void __launch_bounds__(CP_THREADS) k_mx4_quantize(long long R, int K, Tiling t, const float* __restrict__ x,
                                                              long long stride, uint32_t* __restrict__ codes,
                                                              uint8_t* __restrict__ scales) {
-    const int nb = mx_blocks(K), nw = mx_words(K);
-    const long long total = R * nb * 4;
-    const int sub = threadIdx.x & 3;
-    for (long long t = (long long)blockIdx.x * CP_THREADS + threadIdx.x; t < total;
-         t += (long long)gridDim.x * CP_THREADS) {  // whole quads stay together: total % 4 == 0
-        const long long q = t >> 2;
-        const long long row = q / nb;
-        const int b = (int)(q - row * nb);
-        const int k0 = b * GSR_MX_BLOCK + sub * 8;
-        const float* p = x + row * stride + k0;
-        float v[8];
-        uint32_t m = 0;
+    const int nw = mx_words(K), sub = threadIdx.x & 3;
+    v4a lo[MXQ_PER], hi[MXQ_PER];
+    long long row[MXQ_PER];
+    int b[MXQ_PER];
+    bool in[MXQ_PER];  // the same for the four
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = k0 + j < K ? p[j] : 0.0f;
-            const uint32_t a = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-            m = m > a ? m : a;
-        }
+    for (int u = 0; u < MXQ_PER; ++u) {
+        in[u] = tiling_place<MXQ_SPAN>(t, blockIdx.x, u * (CP_THREADS / 4) + (threadIdx.x >> 2), R, row[u], b[u]);
+        const int k0 = b[u] * GSR_MX_BLOCK + sub * 8;
+        const float* p = x + row[u] * stride + k0;
+        const int end = in[u] ? K : 0;
+        lo[u] = load4(p, k0, end);
+        hi[u] = load4(p + 4, k0 + 4, end);
+    }
+#pragma unroll
+    for (int u = 0; u < MXQ_PER; ++u) {
+        uint32_t m = max_bits(max_bits(0u, lo[u]), hi[u]);
         uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true);  // quad_perm 1 0 3 2
         m = m > o ? m : o;
         o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true);  // quad_perm 2 3 0 1
         m = m > o ? m : o;
         const uint32_t s = mx_scale_byte(m);
-        if (k0 < K) codes[row * nw + b * 4 + sub] = s == 255u ? 0u : mx_encode8(v, mx_scale(s));
-        if (sub == 0) scales[row * nb + b] = (uint8_t)s;
+        const int w = b[u] * 4 + sub;
+        if (in[u] && w < nw) codes[row[u] * nw + w] = s == 255u ? 0u : mx_encode8(lo[u], hi[u], mx_scale(s));
+        if (in[u] && sub == 0) scales[row[u] * t.units + b[u]] = (uint8_t)s;
     }
 }
 
-__global__ void __launch_bounds__(CP_THREADS) k_mx4_dequantize(long long R, int K, const uint32_t* __restrict__ codes,
+// Four values (a half word of codes) per lane: a wave writes 1 KB in one piece.
+__global__ void __launch_bounds__(CP_THREADS) k_mx4_dequantize(long long R, int K, Tiling t,
+                                                               const uint16_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales,
                                                                float* __restrict__ x) {
-    const int nb = mx_blocks(K), nw = mx_words(K);
-    const long long total = R * nw;
-    for (long long t = (long long)blockIdx.x * CP_THREADS + threadIdx.x; t < total;
-         t += (long long)gridDim.x * CP_THREADS) {
-        const long long row = t / nw;
-        const int w = (int)(t - row * nw);
-        float v[8];
-        mx_decode8(codes[t], mx_scale(scales[row * nb + (w >> 2)]), v);
-        float* p = x + row * K + w * 8;
+    const int nb = mx_blocks(K), nh = 2 * mx_words(K);
+    long long row;
+    int h;
+    if (!tiling_place<CP_THREADS>(t, blockIdx.x, threadIdx.x, R, row, h)) return;
+    const uint32_t w = codes[row * nh + h];
+    const float s = mx_scale(scales[row * nb + (h >> 3)]);
+    const f2v a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0);
+    const f2v b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+    float* p = x + row * K + 4 * h;
+    if (4 * h + 4 <= K) {
+        *reinterpret_cast<v4a*>(p) = v4a{a.x, a.y, b.x, b.y};
+    } else {
+        const float v[3] = {a.x, a.y, b.x};
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (w * 8 + j < K) p[j] = v[j];
+        for (int j = 0; j < 3; ++j)
+            if (4 * h + j < K) p[j] = v[j];
     }
 }
 
@@ -157,22 +215,6 @@ __device__ __forceinline__ void sh_grad(float x, float y, float z, const float* 
     }
 }
 
-// Decoded coefficients of one Gaussian, 3 floats each, coefficient 0 the constant one.
-template <int DEG>
-struct Coef {
-    static constexpr int N = (DEG + 1) * (DEG + 1);
-    static constexpr int WORDS = (3 * (N - 1) + 7) / 8;
-    float q[8 * WORDS + 3];
-    __device__ __forceinline__ void load(int i, int pitch, int nb, const float* __restrict__ dc, long long dc_stride,
-                                         const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales) {
-        const float* d = dc + i * dc_stride;
-        q[0] = d[0]; q[1] = d[1]; q[2] = d[2];
-#pragma unroll
-        for (int w = 0; w < WORDS; ++w)
-            mx_decode8(codes[(long long)i * pitch + w], mx_scale(scales[(long long)i * nb + (w >> 2)]), q + 3 + 8 * w);
-    }
-};
-
 struct ShArgs {
     int P, V, pitch, nb, M;
     const float* xyz;
@@ -181,6 +223,48 @@ struct ShArgs {
     const uint32_t* codes;
     const uint8_t* scales;
     const float* campos;
+};
+
+struct v3a {  // (a struct: a vector of three would be stored as four)
+    float x, y, z;
+};
+__device__ __forceinline__ v3a load3(const float* p) { return {p[0], p[1], p[2]}; }
+__device__ __forceinline__ void store3(float* p, float x, float y, float z) {
+    p[0] = x; p[1] = y; p[2] = z;
+}
+
+// Decoded coefficients of one Gaussian, 3 floats each, coefficient 0 the constant one.
+template <int DEG>
+struct Coef {
+    static constexpr int N = (DEG + 1) * (DEG + 1);
+    static constexpr int WORDS = (3 * (N - 1) + 7) / 8;   // code words that the degree needs
+    static constexpr int BLOCKS = (3 * (N - 1) + GSR_MX_BLOCK - 1) / GSR_MX_BLOCK;
+    float q[8 * WORDS + 3];
+    __device__ __forceinline__ void load(int i, const ShArgs& a) {
+        const v3a d = load3(a.dc + i * a.dc_stride);
+        q[0] = d.x; q[1] = d.y; q[2] = d.z;
+        uint32_t w[WORDS + 1];
+#pragma unroll
+        for (int k = 0; k < WORDS; ++k) w[k] = a.codes[(long long)i * a.pitch + k];
+#pragma unroll
+        for (int k = 0; k < BLOCKS; ++k) {
+            const float scale = mx_scale(a.scales[(long long)i * a.nb + k]);
+#pragma unroll
+            for (int j = 4 * k; j < 4 * k + 4; ++j)
+                if (j < WORDS) mx_decode8(w[j], scale, q + 3 + 8 * j);
+        }
+    }
+    // The value before the clamp for basis values b: smallest terms first.
+    template <typename F>
+    __device__ __forceinline__ void sum(const F* b, F* s) const {
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            F t = 0;
+#pragma unroll
+            for (int k = N - 1; k >= 0; --k) t += b[k] * (F)q[3 * k + j];
+            s[j] = t + (F)0.5;
+        }
+    }
 };
 
 // u -> u / |u|; returns 1 / |u|, 0 (and d = 0) where u is 0.
@@ -197,57 +281,185 @@ __device__ __forceinline__ float normalize3(float& x, float& y, float& z) {
     return r / m;
 }
 
+// Colours of one Gaussian in every view.
+template <int DEG>
+__device__ __forceinline__ void write_colors(const ShArgs& a, int i, v3a p, const Coef<DEG>& c,
+                                             float* __restrict__ colors) {
+    for (int v = 0; v < a.V; ++v) {
+        float x = p.x - a.campos[3 * v], y = p.y - a.campos[3 * v + 1], z = p.z - a.campos[3 * v + 2];
+        normalize3(x, y, z);
+        float b[Coef<DEG>::N], s[3];
+        sh_values<DEG, float>(x, y, z, b);
+        c.sum(b, s);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) s[j] = s[j] < 0.0f ? 0.0f : s[j];  // keeps a NaN
+        store3(colors + ((long long)v * a.P + i) * 3, s[0], s[1], s[2]);
+    }
+}
+
+// One thread per Gaussian, its coefficients in registers for all views.  Bound by memory with
+// one view (62 bytes a Gaussian at degree 3), by the vector units with many.
 template <int DEG>
 __global__ void __launch_bounds__(CP_THREADS) k_sh_colors(ShArgs a, float* __restrict__ colors) {
     const int i = blockIdx.x * CP_THREADS + threadIdx.x;
     if (i >= a.P) return;
+    const v3a p = load3(a.xyz + 3LL * i);
     Coef<DEG> c;
-    c.load(i, a.pitch, a.nb, a.dc, a.dc_stride, a.codes, a.scales);
-    const float px = a.xyz[3LL * i], py = a.xyz[3LL * i + 1], pz = a.xyz[3LL * i + 2];
-    for (int v = 0; v < a.V; ++v) {
-        float x = px - a.campos[3 * v], y = py - a.campos[3 * v + 1], z = pz - a.campos[3 * v + 2];
-        normalize3(x, y, z);
-        float b[Coef<DEG>::N];
-        sh_values<DEG, float>(x, y, z, b);
-        float s[3] = {0.5f, 0.5f, 0.5f};
+    c.load(i, a);
+    write_colors<DEG>(a, i, p, c, colors);
+}
+
+// ---- rows of features through LDS ------------------------------------------------
+// A wave's 64 rows of 3 M floats lie in one piece of memory, a lane works on one row: the piece
+// moves as float4s of consecutive lanes and turns in the wave's own part of LDS (no block
+// barrier: a wave's LDS operations are in order, a wait for them is enough).  M = 16: rows 13
+// float4s apart, which spreads a lane-per-row access over all banks; other M: rows as they lie.
+constexpr int ROW16 = 13;                  // float4s
+constexpr int ROWS_LDS = 64 * 4 * ROW16;   // floats a wave (also 64 rows of 45)
+__device__ __forceinline__ void wave_lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ void rows_in(const float* __restrict__ src, int rows, int F, float* lds, int lane) {
+    if (F == 48) {
+        v4a v[12];
 #pragma unroll
-        for (int k = 0; k < Coef<DEG>::N; ++k)
+        for (int r = 0; r < 12; ++r) {
+            const int f = lane + 64 * r;
+            v[r] = f / 12 < rows ? *reinterpret_cast<const v4a*>(src + 4 * f) : v4a{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        float4* d = reinterpret_cast<float4*>(lds);
 #pragma unroll
-            for (int j = 0; j < 3; ++j) s[j] += b[k] * c.q[3 * k + j];
-        float* o = colors + ((long long)v * a.P + i) * 3;
-#pragma unroll
-        for (int j = 0; j < 3; ++j) o[j] = s[j] < 0.0f ? 0.0f : s[j];  // keeps a NaN
+        for (int r = 0; r < 12; ++r) {
+            const int f = lane + 64 * r;
+            d[f / 12 * ROW16 + f % 12] = make_float4(v[r].x, v[r].y, v[r].z, v[r].w);
+        }
+    } else {
+        const int n = (rows < 64 ? rows : 64) * F;
+        for (int f = 4 * lane; f < n; f += 256) {
+            const v4a v = load4(src + f, f, n);
+            *reinterpret_cast<float4*>(lds + f) = make_float4(v.x, v.y, v.z, v.w);
+        }
     }
+    wave_lds_wait();
+}
+
+__device__ __forceinline__ void rows_out(float* __restrict__ dst, int rows, int F, const float* lds, int lane) {
+    wave_lds_wait();
+    if (F == 48) {
+        const float4* d = reinterpret_cast<const float4*>(lds);
+#pragma unroll
+        for (int r = 0; r < 12; ++r) {
+            const int f = lane + 64 * r;
+            const float4 v = d[f / 12 * ROW16 + f % 12];
+            if (f / 12 < rows) *reinterpret_cast<v4a*>(dst + 4 * f) = v4a{v.x, v.y, v.z, v.w};
+        }
+    } else {
+        const int n = (rows < 64 ? rows : 64) * F;
+        for (int f = 4 * lane; f < n; f += 256) {
+            const float4 v = *reinterpret_cast<const float4*>(lds + f);
+            if (f + 4 <= n) {
+                *reinterpret_cast<v4a*>(dst + f) = v4a{v.x, v.y, v.z, v.w};
+            } else {
+                dst[f] = v.x;
+                if (f + 1 < n) dst[f + 1] = v.y;
+                if (f + 2 < n) dst[f + 2] = v.z;
+            }
+        }
+    }
+}
+
+// Training forward: a Gaussian's fp32 coefficients are read once, rounded to codes (kept for the
+// backward), read back and evaluated.  The blocks that the degree touches are rounded whole, so a
+// code does not depend on the degree.
+template <int DEG>
+__global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, const float* __restrict__ features,
+                                                                   uint32_t* __restrict__ codes,
+                                                                   uint8_t* __restrict__ scales,
+                                                                   float* __restrict__ colors) {
+    using C = Coef<DEG>;
+    __shared__ float4 s_rows[CP_THREADS / 64][ROWS_LDS / 4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int first = blockIdx.x * CP_THREADS + wave * 64, i = first + lane, F = 3 * a.M;
+    if (first >= a.P) return;  // the whole wave
+    float* lds = reinterpret_cast<float*>(s_rows[wave]);
+    rows_in(features + (long long)first * F, a.P - first, F, lds, lane);
+    if (i >= a.P) return;
+    constexpr int VALUES = C::BLOCKS * GSR_MX_BLOCK;  // of the row behind its constant coefficient
+    float v[VALUES + 3];
+    if (F == 48) {
+        const float4* d = reinterpret_cast<const float4*>(lds) + lane * ROW16;
+#pragma unroll
+        for (int k = 0; k < 12; ++k) {
+            const float4 t = d[k];
+            const float e[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (4 * k + j < VALUES + 3) v[4 * k + j] = e[j];
+        }
+#pragma unroll
+        for (int k = 48; k < VALUES + 3; ++k) v[k] = 0.0f;
+    } else {
+#pragma unroll
+        for (int k = 0; k < VALUES + 3; ++k) v[k] = k < F ? lds[lane * F + k] : 0.0f;
+    }
+    const v3a p = load3(a.xyz + 3LL * i);
+    C c;
+    c.q[0] = v[0]; c.q[1] = v[1]; c.q[2] = v[2];
+    uint32_t w[C::WORDS + 1], bytes = 0;
+#pragma unroll
+    for (int b = 0; b < C::BLOCKS; ++b) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < GSR_MX_BLOCK; ++k) {
+            const uint32_t x = __float_as_uint(v[3 + b * GSR_MX_BLOCK + k]) & 0x7FFFFFFFu;
+            m = m > x ? m : x;
+        }
+        const uint32_t sb = mx_scale_byte(m);
+        bytes |= sb << (8 * b);
+#pragma unroll
+        for (int j = 4 * b; j < 4 * b + 4; ++j)
+            if (j < C::WORDS) {
+                const float* x = v + 3 + 8 * j;
+                w[j] = sb == 255u ? 0u : mx_encode8(v4a{x[0], x[1], x[2], x[3]}, v4a{x[4], x[5], x[6], x[7]},
+                                                    mx_scale(sb));
+                mx_decode8(w[j], mx_scale(sb), c.q + 3 + 8 * j);
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < C::WORDS; ++j) codes[(long long)i * a.pitch + j] = w[j];
+#pragma unroll
+    for (int b = 0; b < C::BLOCKS; ++b) scales[(long long)i * a.nb + b] = (uint8_t)(bytes >> (8 * b));
+    write_colors<DEG>(a, i, p, c, colors);
 }
 
 // The value before the clamp in 64 bits.
 template <int DEG>
-__device__ void preclamp64(const Coef<DEG>& c, float px, float py, float pz, const float* cam, double* s) {
-    const double x = (double)px - cam[0], y = (double)py - cam[1], z = (double)pz - cam[2];
+__device__ __forceinline__ void preclamp64(const Coef<DEG>& c, v3a p, const float* cam, double* s) {
+    const double x = (double)p.x - cam[0], y = (double)p.y - cam[1], z = (double)p.z - cam[2];
     const double n = x * x + y * y + z * z;
     const double r = n > 0.0 ? 1.0 / sqrt(n) : 0.0;
     double b[Coef<DEG>::N];
     sh_values<DEG, double>(x * r, y * r, z * r, b);
-    s[0] = s[1] = s[2] = 0.5;
-#pragma unroll
-    for (int k = 0; k < Coef<DEG>::N; ++k)
-#pragma unroll
-        for (int j = 0; j < 3; ++j) s[j] += b[k] * (double)c.q[3 * k + j];
+    c.template sum<double>(b, s);
 }
 
-template <int DEG>
+// One thread per Gaussian, all views; the features' gradient rows leave through LDS.
+// WANT_F: dfeatures is wanted (else at most its first coefficient, ddc).
+template <int DEG, bool WANT_F>
 __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, const float* __restrict__ dcolors,
                                                                    float* __restrict__ dxyz, float* __restrict__ ddc,
                                                                    float* __restrict__ dfeatures) {
-    constexpr int N = Coef<DEG>::N;
-    const int i = blockIdx.x * CP_THREADS + threadIdx.x;
-    if (i >= a.P) return;
+    constexpr int N = Coef<DEG>::N, NF = WANT_F ? N : 1;
+    __shared__ float4 s_rows[WANT_F ? CP_THREADS / 64 : 1][WANT_F ? ROWS_LDS / 4 : 1];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int first = blockIdx.x * CP_THREADS + wave * 64;
+    if (first >= a.P) return;                                 // the whole wave
+    const int i = first + lane < a.P ? first + lane : a.P - 1;  // lanes behind the end repeat the last row
+    const v3a p = load3(a.xyz + 3LL * i);
     Coef<DEG> c;
-    c.load(i, a.pitch, a.nb, a.dc, a.dc_stride, a.codes, a.scales);
-    const float px = a.xyz[3LL * i], py = a.xyz[3LL * i + 1], pz = a.xyz[3LL * i + 2];
-    // Rounding of the value before the clamp: a direction is good to 3 ulp of 1, a basis value
-    // (slope at most 4) to 32, so a channel's sum to 2^-19 of its coefficients' sum; inside twice
-    // that the sign is taken from 64 bits.
+    c.load(i, a);
+    // Rounding of the value before the clamp, in units of 2^-24: a direction is good to 6, a basis
+    // value (slope at most 4.9) to 37, the sum of 16 products to 53 of the coefficients' sum; nearer to
+    // zero than 64 the sign is taken from 64 bits, so that no gradient hangs on a rounding.
     float near[3] = {0.5f, 0.5f, 0.5f};
 #pragma unroll
     for (int k = 0; k < N; ++k)
@@ -255,20 +467,18 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, con
         for (int j = 0; j < 3; ++j) near[j] += fabsf(c.q[3 * k + j]);
 #pragma unroll
     for (int j = 0; j < 3; ++j) near[j] *= 0x1p-18f;
-    float acc[3 * N];
+    float acc[3 * NF];
 #pragma unroll
-    for (int k = 0; k < 3 * N; ++k) acc[k] = 0.0f;
+    for (int k = 0; k < 3 * NF; ++k) acc[k] = 0.0f;
     float ax = 0.0f, ay = 0.0f, az = 0.0f;
     for (int v = 0; v < a.V; ++v) {
         const float* cam = a.campos + 3 * v;
-        float x = px - cam[0], y = py - cam[1], z = pz - cam[2];
+        const v3a gp = load3(dcolors + ((long long)v * a.P + i) * 3);
+        float x = p.x - cam[0], y = p.y - cam[1], z = p.z - cam[2];
         const float r = normalize3(x, y, z);
-        float b[N], s[3] = {0.5f, 0.5f, 0.5f};
+        float b[N], s[3];
         sh_values<DEG, float>(x, y, z, b);
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-#pragma unroll
-            for (int j = 0; j < 3; ++j) s[j] += b[k] * c.q[3 * k + j];
+        c.sum(b, s);
         bool on[3];
         bool close = false;
 #pragma unroll
@@ -278,39 +488,44 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, con
         }
         if (close) {
             double t[3];
-            preclamp64<DEG>(c, px, py, pz, cam, t);
+            preclamp64<DEG>(c, p, cam, t);
 #pragma unroll
             for (int j = 0; j < 3; ++j) on[j] = t[j] >= 0.0;
         }
-        const float* gp = dcolors + ((long long)v * a.P + i) * 3;
-        float g[3];
+        const float g[3] = {on[0] ? gp.x : 0.0f, on[1] ? gp.y : 0.0f, on[2] ? gp.z : 0.0f};
 #pragma unroll
-        for (int j = 0; j < 3; ++j) g[j] = on[j] ? gp[j] : 0.0f;
-        float w[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            w[k] = c.q[3 * k] * g[0] + c.q[3 * k + 1] * g[1] + c.q[3 * k + 2] * g[2];
+        for (int k = 0; k < NF; ++k)
 #pragma unroll
             for (int j = 0; j < 3; ++j) acc[3 * k + j] += b[k] * g[j];
+        if (DEG > 0 && dxyz) {
+            float w[N], gx, gy, gz;
+#pragma unroll
+            for (int k = 0; k < N; ++k) w[k] = c.q[3 * k] * g[0] + c.q[3 * k + 1] * g[1] + c.q[3 * k + 2] * g[2];
+            sh_grad<DEG>(x, y, z, w, gx, gy, gz);
+            const float along = gx * x + gy * y + gz * z;
+            ax += r * (gx - along * x);
+            ay += r * (gy - along * y);
+            az += r * (gz - along * z);
         }
-        float gx, gy, gz;
-        sh_grad<DEG>(x, y, z, w, gx, gy, gz);
-        const float along = gx * x + gy * y + gz * z;
-        ax += r * (gx - along * x);
-        ay += r * (gy - along * y);
-        az += r * (gz - along * z);
     }
-    if (dxyz) {
-        dxyz[3LL * i] = ax; dxyz[3LL * i + 1] = ay; dxyz[3LL * i + 2] = az;
+    if (first + lane < a.P) {
+        if (dxyz) store3(dxyz + 3LL * i, ax, ay, az);
+        if (ddc) store3(ddc + 3LL * i, acc[0], acc[1], acc[2]);
     }
-    if (ddc)
+    if constexpr (WANT_F) {
+        const int F = 3 * a.M;
+        float* lds = reinterpret_cast<float*>(s_rows[wave]);
+        if (F == 48) {
+            float4* d = reinterpret_cast<float4*>(lds) + lane * ROW16;
+            auto at = [&](int k) { return k < 3 * N ? acc[k] : 0.0f; };
 #pragma unroll
-        for (int j = 0; j < 3; ++j) ddc[3LL * i + j] = acc[j];
-    if (dfeatures) {
-        float* o = dfeatures + 3LL * a.M * i;
+            for (int k = 0; k < 12; ++k) d[k] = make_float4(at(4 * k), at(4 * k + 1), at(4 * k + 2), at(4 * k + 3));
+        } else {
 #pragma unroll
-        for (int k = 0; k < 3 * N; ++k) o[k] = acc[k];
-        for (int k = 3 * N; k < 3 * a.M; ++k) o[k] = 0.0f;
+            for (int k = 0; k < 3 * N; ++k) lds[lane * F + k] = acc[k];
+            for (int k = 3 * N; k < F; ++k) lds[lane * F + k] = 0.0f;
+        }
+        rows_out(dfeatures + (long long)first * F, a.P - first, F, lds, lane);
     }
 }
 
@@ -541,25 +756,64 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
 }
 
 // ------------------------------------------------------------------------ rows --
-constexpr int TAKE_MAX = 32;
-struct TakeArgs {
-    gsr_rows t[TAKE_MAX];
+// A copy: K rows of each tensor read and written once, bound by memory.  A block moves
+// TAKE_SPAN units of one tensor's output, a unit being 16 bytes where the rows are whole
+// float4s (the features, 48 of a Gaussian's 61 floats, and the rotations), else 4.
+constexpr int TAKE_MAX = 32;    // tensors a launch
+constexpr int TAKE_PER = 4;     // units a thread: their ids, then their values, are in flight together
+constexpr int TAKE_SPAN = CP_THREADS * TAKE_PER;
+struct TakeTensor {
+    const void* src;
+    void* dst;
+    Tiling t;
+    int K;  // rows to write (0 where they are 0 wide)
+    int rows, vec, pad;
+    uint32_t block0, blocks;  // first block, how many
 };
-__global__ void __launch_bounds__(CP_THREADS) k_take_rows(TakeArgs a, int K, const int* __restrict__ ids) {
-    const gsr_rows t = a.t[blockIdx.y];
-    const uint32_t* src = static_cast<const uint32_t*>(t.src);
-    uint32_t* dst = static_cast<uint32_t*>(t.dst);
-    const long long n = (long long)K * t.width;
-    for (long long e = (long long)blockIdx.x * CP_THREADS + threadIdx.x; e < n + t.pad;
-         e += (long long)gridDim.x * CP_THREADS) {
-        uint32_t v = 0;
-        if (e < n) {
-            const int row = (int)(e / t.width);
+struct TakeArgs {
+    int n;
+    TakeTensor t[TAKE_MAX];
+};
+
+template <typename V>
+__device__ __forceinline__ void take_block(const TakeTensor& t, uint32_t block, const int* __restrict__ ids) {
+    const V* src = static_cast<const V*>(t.src);
+    V* dst = static_cast<V*>(t.dst);
+    long long to[TAKE_PER], from[TAKE_PER];
+#pragma unroll
+    for (int k = 0; k < TAKE_PER; ++k) {
+        long long row;
+        int unit;
+        to[k] = from[k] = -1;
+        if (tiling_place<TAKE_SPAN>(t.t, block, k * CP_THREADS + threadIdx.x, t.K, row, unit)) {
+            to[k] = row * t.t.units + unit;
             const int id = ids[row];
-            if ((unsigned)id < (unsigned)t.rows) v = src[(long long)id * t.width + (e - (long long)row * t.width)];
+            if ((unsigned)id < (unsigned)t.rows) from[k] = (long long)id * t.t.units + unit;
         }
-        dst[e] = v;
     }
+    V v[TAKE_PER];
+#pragma unroll
+    for (int k = 0; k < TAKE_PER; ++k) v[k] = from[k] >= 0 ? src[from[k]] : V{};
+#pragma unroll
+    for (int k = 0; k < TAKE_PER; ++k)
+        if (to[k] >= 0) dst[to[k]] = v[k];
+    if (t.pad > 0 && block == t.blocks - 1) {  // the words behind the last row
+        uint32_t* tail = reinterpret_cast<uint32_t*>(dst + (long long)t.K * t.t.units);
+        for (int k = threadIdx.x; k < t.pad; k += CP_THREADS) tail[k] = 0u;
+    }
+}
+
+__global__ void __launch_bounds__(CP_THREADS) k_take_rows(TakeArgs a, const int* __restrict__ ids) {
+    int lo = 0, hi = a.n - 1;
+    while (lo < hi) {
+        const int m = (lo + hi + 1) >> 1;
+        if (a.t[m].block0 <= blockIdx.x) lo = m;
+        else hi = m - 1;
+    }
+    const TakeTensor t = a.t[lo];
+    const uint32_t block = blockIdx.x - t.block0;
+    if (t.vec == 4) take_block<uint4>(t, block, ids);
+    else take_block<uint32_t>(t, block, ids);
 }
 
 unsigned grid_for(long long items, long long cap) {
@@ -600,8 +854,10 @@ GSR_API int gsr_mx4_quantize(long long R, int K, const float* x, long long row_s
     if (R == 0 || K == 0) return 0;
     if (!x || !codes || !scales) return set_error("[gsr] gsr_mx4_quantize: null buffer");
     if (row_stride < K && R > 1) return set_error("[gsr] gsr_mx4_quantize: rows overlap");
-    k_mx4_quantize<<<grid_for(R * mx_blocks(K) * 4, 1 << 20), CP_THREADS, 0, (hipStream_t)stream>>>(
-        R, K, x, row_stride, codes, scales);
+    const Tiling t = tiling(mx_blocks(K), MXQ_SPAN);
+    const long long blocks = tiling_blocks(t, R, MXQ_SPAN);
+    if (blocks >= (1LL << 31)) return set_error("[gsr] gsr_mx4_quantize: too many rows in one call");
+    k_mx4_quantize<<<(unsigned)blocks, CP_THREADS, 0, (hipStream_t)stream>>>(R, K, t, x, row_stride, codes, scales);
     return launched("mx4_quantize");
 }
 
@@ -610,8 +866,11 @@ GSR_API int gsr_mx4_dequantize(long long R, int K, const uint32_t* codes, const 
     if (int rc = check_rows(R, K)) return rc;
     if (R == 0 || K == 0) return 0;
     if (!x || !codes || !scales) return set_error("[gsr] gsr_mx4_dequantize: null buffer");
-    k_mx4_dequantize<<<grid_for(R * mx_words(K), 1 << 20), CP_THREADS, 0, (hipStream_t)stream>>>(R, K, codes, scales,
-                                                                                              x);
+    const Tiling t = tiling((K + 3) / 4, CP_THREADS);
+    const long long blocks = tiling_blocks(t, R, CP_THREADS);
+    if (blocks >= (1LL << 31)) return set_error("[gsr] gsr_mx4_dequantize: too many rows in one call");
+    k_mx4_dequantize<<<(unsigned)blocks, CP_THREADS, 0, (hipStream_t)stream>>>(
+        R, K, t, reinterpret_cast<const uint16_t*>(codes), scales, x);
     return launched("mx4_dequantize");
 }
 
@@ -631,6 +890,22 @@ GSR_API int gsr_sh_colors(int P, int V, int degree, int M, const float* xyz, con
     return launched("sh_colors");
 }
 
+GSR_API int gsr_sh_colors_quantize(int P, int V, int degree, int M, const float* xyz, const float* features,
+                                   const float* campos, uint32_t* codes, uint8_t* scales, float* colors,
+                                   void* stream) {
+    if (int rc = check_colors(P, V, degree, M, xyz, features, codes, scales, campos)) return rc;
+    if (P == 0) return 0;
+    if (!colors) return set_error("[gsr] gsr_sh_colors_quantize: null buffer");
+    const ShArgs a = sh_args(P, V, M, xyz, nullptr, 0, nullptr, nullptr, campos);
+    const unsigned grid = grid_for(P, 1LL << 31);
+    hipStream_t st = (hipStream_t)stream;
+    if (degree == 0) k_sh_colors_quantize<0><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, colors);
+    else if (degree == 1) k_sh_colors_quantize<1><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, colors);
+    else if (degree == 2) k_sh_colors_quantize<2><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, colors);
+    else k_sh_colors_quantize<3><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, colors);
+    return launched("sh_colors_quantize");
+}
+
 GSR_API int gsr_sh_colors_backward(int P, int V, int degree, int M, const float* xyz, const float* dc,
                                    long long dc_stride, const uint32_t* codes, const uint8_t* scales,
                                    const float* campos, const float* dcolors, float* dxyz, float* ddc,
@@ -641,10 +916,14 @@ GSR_API int gsr_sh_colors_backward(int P, int V, int degree, int M, const float*
     const ShArgs a = sh_args(P, V, M, xyz, dc, dc_stride, codes, scales, campos);
     const unsigned grid = grid_for(P, 1LL << 31);
     hipStream_t st = (hipStream_t)stream;
-    if (degree == 0) k_sh_colors_backward<0><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures);
-    else if (degree == 1) k_sh_colors_backward<1><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures);
-    else if (degree == 2) k_sh_colors_backward<2><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures);
-    else k_sh_colors_backward<3><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures);
+#define GSR_SH_BACKWARD(D)                                                                              \
+    if (dfeatures) k_sh_colors_backward<D, true><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures); \
+    else k_sh_colors_backward<D, false><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures)
+    if (degree == 0) { GSR_SH_BACKWARD(0); }
+    else if (degree == 1) { GSR_SH_BACKWARD(1); }
+    else if (degree == 2) { GSR_SH_BACKWARD(2); }
+    else { GSR_SH_BACKWARD(3); }
+#undef GSR_SH_BACKWARD
     return launched("sh_colors_backward");
 }
 
@@ -701,7 +980,8 @@ GSR_API int gsr_take_rows(int K, const int* ids, int n, const gsr_rows* tensors,
         return set_error("[gsr] gsr_take_rows: invalid arguments");
     for (int k = 0; k < n; ++k) {
         const gsr_rows& t = tensors[k];
-        if (t.width < 0 || t.rows < 0 || t.pad < 0) return set_error("[gsr] gsr_take_rows: invalid width or rows");
+        if (t.width < 0 || t.width > (1 << 20) || t.rows < 0 || t.pad < 0)
+            return set_error("[gsr] gsr_take_rows: invalid width or rows");
         const long long words = (long long)K * t.width;
         if ((words > 0 && t.rows > 0 && !t.src) || (words + t.pad > 0 && !t.dst))
             return set_error("[gsr] gsr_take_rows: null buffer");
@@ -710,15 +990,21 @@ GSR_API int gsr_take_rows(int K, const int* ids, int n, const gsr_rows* tensors,
     bool any = false;
     for (int k0 = 0; k0 < n; k0 += TAKE_MAX) {
         TakeArgs a{};
-        const int m = n - k0 < TAKE_MAX ? n - k0 : TAKE_MAX;
-        long long most = 0;
-        for (int k = 0; k < m; ++k) {
-            a.t[k] = tensors[k0 + k];
-            most = std::max(most, (long long)K * a.t[k].width + a.t[k].pad);
+        long long blocks = 0;
+        for (int k = k0; k < n && k < k0 + TAKE_MAX; ++k) {
+            const gsr_rows& q = tensors[k];
+            const bool wide = q.width % 4 == 0 && ((uintptr_t)q.src | (uintptr_t)q.dst) % 16 == 0;
+            if ((long long)K * q.width + q.pad == 0) continue;
+            const Tiling t = tiling(std::max(1, wide ? q.width / 4 : q.width), TAKE_SPAN);
+            const int rows = q.width > 0 ? K : 0;
+            const long long nb = std::max(1LL, tiling_blocks(t, rows, TAKE_SPAN));
+            a.t[a.n++] = {q.src, q.dst, t, rows, q.rows, wide ? 4 : 1, q.pad, (uint32_t)blocks, (uint32_t)nb};
+            blocks += nb;
+            if (blocks >= (1LL << 31)) return set_error("[gsr] gsr_take_rows: too many rows in one call");
         }
-        if (most == 0) continue;
+        if (a.n == 0) continue;
         any = true;
-        k_take_rows<<<dim3(grid_for(most, 1 << 16), m), CP_THREADS, 0, st>>>(a, K, ids);
+        k_take_rows<<<(unsigned)blocks, CP_THREADS, 0, st>>>(a, ids);
     }
     return any ? launched("take_rows") : 0;
 }

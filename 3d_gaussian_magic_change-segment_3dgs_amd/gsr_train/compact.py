@@ -42,6 +42,7 @@ class _Rows(ctypes.Structure):
 for _name, _args in (("gsr_mx4_quantize", [_ll, _i, _vp, _ll, _vp, _vp, _vp]),
                      ("gsr_mx4_dequantize", [_ll, _i, _vp, _vp, _vp, _vp]),
                      ("gsr_sh_colors", [_i, _i, _i, _i, _vp, _vp, _ll, _vp, _vp, _vp, _vp, _vp]),
+                     ("gsr_sh_colors_quantize", [_i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
                      ("gsr_sh_colors_backward", [_i, _i, _i, _i, _vp, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
                      ("gsr_accumulate_weights", [_i, _vp, _ll, _f, _vp, _vp]),
                      ("gsr_keep_heaviest", [_i, _vp, _i, ctypes.POINTER(_Group), _vp, _vp, _vp]),
@@ -51,7 +52,8 @@ for _name, _args in (("gsr_mx4_quantize", [_ll, _i, _vp, _ll, _vp, _vp, _vp]),
 _lib.gsr_keep_ws_bytes.restype = ctypes.c_size_t
 _lib.gsr_keep_ws_bytes.argtypes = [_i]
 
-EXPORTED_SYMBOLS = ("gsr_mx4_quantize", "gsr_mx4_dequantize", "gsr_sh_colors", "gsr_sh_colors_backward",
+EXPORTED_SYMBOLS = ("gsr_mx4_quantize", "gsr_mx4_dequantize", "gsr_sh_colors", "gsr_sh_colors_quantize",
+                    "gsr_sh_colors_backward",
                     "gsr_accumulate_weights", "gsr_keep_ws_bytes", "gsr_keep_heaviest", "gsr_take_rows")
 
 
@@ -187,8 +189,13 @@ class _ShColorsQuantized(torch.autograd.Function):
     @staticmethod
     def forward(ctx, xyz, features, campos, degree, single):
         P, M = features.shape[:2]
-        codes, scales = _quantize(features.view(P, 3 * M)[:, 3:])
-        colors = _forward(xyz, features[:, 0], campos, codes, scales, degree, M, single)
+        K, V, dev = 3 * (M - 1), campos.shape[0], xyz.device
+        codes = torch.empty((P, 4 * _words(K)), dtype=torch.uint8, device=dev)
+        scales = torch.empty((P, _blocks(K)), dtype=torch.uint8, device=dev)
+        colors = torch.empty((P, 3) if single else (V, P, 3), dtype=torch.float32, device=dev)
+        if P:
+            _call(dev, _lib.gsr_sh_colors_quantize, P, V, degree, M, xyz.data_ptr(), features.data_ptr(),
+                  campos.data_ptr(), codes.data_ptr(), scales.data_ptr(), colors.data_ptr())
         ctx.save_for_backward(xyz, features, campos, codes, scales)
         ctx.degree, ctx.M = degree, M
         return colors

@@ -46,6 +46,12 @@ GSR_API int gsr_mx4_dequantize(long long R, int K, const uint32_t* codes, const 
 GSR_API int gsr_sh_colors(int P, int V, int degree, int M, const float* xyz, const float* dc, long long dc_stride,
                           const uint32_t* codes, const uint8_t* scales, const float* campos, float* colors,
                           void* stream);
+/* The same from fp32 features [P, M, 3] whose coefficients above the constant one are rounded
+ * in the call.  codes / scales: rows of 3 (M - 1) values as gsr_mx4_quantize writes them, of which
+ * those that `degree` reads are written (for gsr_sh_colors_backward of the same degree). */
+GSR_API int gsr_sh_colors_quantize(int P, int V, int degree, int M, const float* xyz, const float* features,
+                                   const float* campos, uint32_t* codes, uint8_t* scales, float* colors,
+                                   void* stream);
 /* Gradients for dcolors [V, P, 3], summed over the views in order; a colour channel
  * takes part where its value before the clamp is >= 0 (the sign is decided in 64
  * bits where 32 cannot).  Each of the outputs may be NULL: dxyz [P, 3] (0 where u is 0);

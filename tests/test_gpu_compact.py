@@ -376,6 +376,22 @@ def test_take_rows_of_ids_outside():
     assert torch.equal(y[0], x[3]) and torch.equal(y[4], x[0]) and (y[1:4] == 0).all() and (z == 0).all()
 
 
+def test_take_rows_wide_and_padded():
+    """Rows wider than a block's span, and the words behind a destination's last row."""
+    from gsr_train import compact as T
+    ids = torch.randint(0, 50, (40,), generator=gen(1), dtype=torch.int32).to(DEV)
+    for width in (1023, 1024, 1025, 1500, 4096, 4100, 9001):
+        x = torch.randn(50, width, generator=gen(width)).to(DEV)
+        assert torch.equal(T.take_rows(ids, [x])[0], x[ids.long()]), width
+    for K, width, pad in ((40, 3, 7), (0, 3, 70), (40, 0, 300), (21, 48, 0), (1, 12, 2000)):
+        x = torch.randn(50, width, generator=gen(2)).to(DEV)
+        buf = torch.full((K * width + pad + 5,), 9.0, device=DEV)
+        table = (T._Rows * 1)((x.data_ptr(), buf.data_ptr(), width, 50, pad))
+        T._call(x.device, T._lib.gsr_take_rows, K, ids.data_ptr(), 1, table)
+        assert torch.equal(buf[:K * width].view(K, width), x[ids[:K].long()])
+        assert (buf[K * width:K * width + pad] == 0).all() and (buf[K * width + pad:] == 9).all()
+
+
 def test_accumulate_weights():
     import gsr_train as G
     w = torch.randn(1001, 3, generator=gen(1)).to(DEV)
