@@ -81,11 +81,21 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
 }
 
 
-// Values [k, k + 4) of a row of K, zeros behind its end.
+// Values [k, k + 4) of a row of K (p: its value k), zeros behind its end.  A piece that ends with
+// the row is read as the row's last four values, shifted: one load whatever the length.
 __device__ __forceinline__ v4a load4(const float* p, int k, int K) {
     v4a r = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (k + 4 <= K) {
-        r = *reinterpret_cast<const v4a*>(p);
+    if ((K & 3) == 0) {
+        if (k < K) r = *reinterpret_cast<const v4a*>(p);
+    } else if (K >= 4) {
+        const int over = k + 4 - K;
+        if (over < 4) {
+            const v4a q = *reinterpret_cast<const v4a*>(over > 0 ? p - over : p);
+            r.x = over <= 0 ? q.x : over == 1 ? q.y : over == 2 ? q.z : q.w;
+            r.y = over <= 0 ? q.y : over == 1 ? q.z : over == 2 ? q.w : 0.0f;
+            r.z = over <= 0 ? q.z : over == 1 ? q.w : 0.0f;
+            r.w = over <= 0 ? q.w : 0.0f;
+        }
     } else {
         if (k < K) r.x = p[0];
         if (k + 1 < K) r.y = p[1];
@@ -159,6 +169,12 @@ __global__ void __launch_bounds__(CP_THREADS) k_mx4_dequantize(long long R, int 
 }
 
 // --------------------------------------------------------------------- colours --
+// No contraction by the compiler from here on: the products that are to be fused say so, and so
+// every kernel that evaluates an expression gets the same bits.
+#pragma clang fp contract(off)
+__device__ __forceinline__ float mad(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double mad(double a, double b, double c) { return __builtin_fma(a, b, c); }
+
 // Real spherical harmonics up to degree 3 in the reference's order and signs
 // (utils/sh_utils.py:26-48); F = float, or double where a sign needs it.
 template <int DEG, typename F>
@@ -170,19 +186,20 @@ __device__ __forceinline__ void sh_values(F x, F y, F z, F* b) {
     }
     if constexpr (DEG > 1) {
         const F a = (F)1.0925484305920792, c = (F)0.31539156525252005, e = (F)0.5462742152960396;
-        const F xx = x * x, yy = y * y, zz = z * z;
-        b[4] = a * (x * y); b[5] = -a * (y * z); b[6] = c * ((F)2 * zz - xx - yy); b[7] = -a * (x * z);
-        b[8] = e * (xx - yy);
+        const F xx = x * x, yy = y * y, zz = z * z, t = xx + yy, d = xx - yy;
+        b[4] = a * (x * y); b[5] = -a * (y * z); b[6] = c * mad((F)2, zz, -t); b[7] = -a * (x * z);
+        b[8] = e * d;
         if constexpr (DEG > 2) {
             const F p = (F)0.5900435899266435, q = (F)2.890611442640554, r = (F)0.4570457994644658,
                     s = (F)0.3731763325901154, u = (F)1.445305721320277;
-            b[9] = -p * y * ((F)3 * xx - yy);
+            const F o = -r * mad((F)4, zz, -t);
+            b[9] = -p * y * mad((F)3, xx, -yy);
             b[10] = q * (x * y) * z;
-            b[11] = -r * y * ((F)4 * zz - xx - yy);
-            b[12] = s * z * ((F)2 * zz - (F)3 * xx - (F)3 * yy);
-            b[13] = -r * x * ((F)4 * zz - xx - yy);
-            b[14] = u * z * (xx - yy);
-            b[15] = -p * x * (xx - (F)3 * yy);
+            b[11] = o * y;
+            b[12] = s * z * mad((F)2, zz, (F)-3 * t);
+            b[13] = o * x;
+            b[14] = u * z * d;
+            b[15] = -p * x * mad((F)-3, yy, xx);
         }
     }
 }
@@ -198,20 +215,32 @@ __device__ __forceinline__ void sh_grad(float x, float y, float z, const float* 
     }
     if constexpr (DEG > 1) {
         const float a = 1.0925484305920792f, c = 0.31539156525252005f, e = 0.5462742152960396f;
-        gx += a * (y * w[4] - z * w[7]) - 2.0f * c * x * w[6] + 2.0f * e * x * w[8];
-        gy += a * (x * w[4] - z * w[5]) - 2.0f * c * y * w[6] - 2.0f * e * y * w[8];
-        gz += -a * (y * w[5] + x * w[7]) + 4.0f * c * z * w[6];
-        if constexpr (DEG > 2) {
-            const float p = 0.5900435899266435f, q = 2.890611442640554f, r = 0.4570457994644658f,
-                        s = 0.3731763325901154f, u = 1.445305721320277f;
-            const float xx = x * x, yy = y * y, zz = z * z, xy = x * y, yz = y * z, xz = x * z;
-            gx += -6.0f * p * xy * w[9] + q * yz * w[10] + 2.0f * r * xy * w[11] - 6.0f * s * xz * w[12] -
-                  r * (4.0f * zz - 3.0f * xx - yy) * w[13] + 2.0f * u * xz * w[14] - 3.0f * p * (xx - yy) * w[15];
-            gy += -3.0f * p * (xx - yy) * w[9] + q * xz * w[10] - r * (4.0f * zz - xx - 3.0f * yy) * w[11] -
-                  6.0f * s * yz * w[12] + 2.0f * r * xy * w[13] - 2.0f * u * yz * w[14] + 6.0f * p * xy * w[15];
-            gz += q * xy * w[10] - 8.0f * r * yz * w[11] + 3.0f * s * (2.0f * zz - xx - yy) * w[12] -
-                  8.0f * r * xz * w[13] + u * (xx - yy) * w[14];
-        }
+        const float w4 = a * w[4], w5 = -a * w[5], w6 = 2.0f * c * w[6], w7 = -a * w[7], w8 = 2.0f * e * w[8];
+        gx = mad(y, w4, mad(z, w7, mad(x, w8 - w6, gx)));
+        gy = mad(x, w4, mad(z, w5, mad(-y, w8 + w6, gy)));
+        gz = mad(y, w5, mad(x, w7, mad(2.0f * z, w6, gz)));
+    }
+    if constexpr (DEG > 2) {
+        const float p = 0.5900435899266435f, q = 2.890611442640554f, r = 0.4570457994644658f,
+                    s = 0.3731763325901154f, u = 1.445305721320277f;
+        const float xx = x * x, yy = y * y, zz = z * z, xy = x * y, yz = y * z, xz = x * z, t = xx + yy, d = xx - yy;
+        const float w9 = 3.0f * p * w[9], w10 = q * w[10], w11 = r * w[11], w12 = 3.0f * s * w[12],
+                    w13 = r * w[13], w14 = u * w[14], w15 = 3.0f * p * w[15];
+        const float z4 = 4.0f * zz;
+        gx = mad(-2.0f * xy, w9 - w11, gx);
+        gx = mad(yz, w10, gx);
+        gx = mad(2.0f * xz, w14 - w12, gx);
+        gx = mad(-(z4 - mad(2.0f, xx, t)), w13, gx);
+        gx = mad(-d, w15, gx);
+        gy = mad(-d, w9, gy);
+        gy = mad(xz, w10, gy);
+        gy = mad(-(z4 - mad(2.0f, yy, t)), w11, gy);
+        gy = mad(-2.0f * yz, w12 + w14, gy);
+        gy = mad(2.0f * xy, w13 + w15, gy);
+        gz = mad(xy, w10, gz);
+        gz = mad(-8.0f * z, mad(y, w11, x * w13), gz);
+        gz = mad(mad(2.0f, zz, -t), w12, gz);
+        gz = mad(d, w14, gz);
     }
 }
 
@@ -241,7 +270,7 @@ struct Coef {
     static constexpr int BLOCKS = (3 * (N - 1) + GSR_MX_BLOCK - 1) / GSR_MX_BLOCK;
     float q[8 * WORDS + 3];
     __device__ __forceinline__ void load(int i, const ShArgs& a) {
-        const v3a d = load3(a.dc + i * a.dc_stride);
+        const v3a d = a.dc ? load3(a.dc + i * a.dc_stride) : v3a{0.0f, 0.0f, 0.0f};
         q[0] = d.x; q[1] = d.y; q[2] = d.z;
         uint32_t w[WORDS + 1];
 #pragma unroll
@@ -261,7 +290,7 @@ struct Coef {
         for (int j = 0; j < 3; ++j) {
             F t = 0;
 #pragma unroll
-            for (int k = N - 1; k >= 0; --k) t += b[k] * (F)q[3 * k + j];
+            for (int k = N - 1; k >= 0; --k) t = mad(b[k], (F)q[3 * k + j], t);
             s[j] = t + (F)0.5;
         }
     }
@@ -269,28 +298,68 @@ struct Coef {
 
 // u -> u / |u|; returns 1 / |u|, 0 (and d = 0) where u is 0.
 __device__ __forceinline__ float normalize3(float& x, float& y, float& z) {
-    float n = x * x + y * y + z * z, m = 1.0f;
+    float n = mad(x, x, mad(y, y, z * z)), m = 1.0f;
     if (!(n > 1e-30f && n < 1e30f)) {  // the squares leave the range (or u is 0, or not finite)
         m = fmaxf(fabsf(x), fmaxf(fabsf(y), fabsf(z)));
         if (!(m > 0.0f)) return 0.0f;
         x /= m; y /= m; z /= m;
-        n = x * x + y * y + z * z;
+        n = mad(x, x, mad(y, y, z * z));
     }
     const float r = 1.0f / sqrtf(n);
     x *= r; y *= r; z *= r;
     return r / m;
 }
 
-// Colours of one Gaussian in every view.
+// The value before the clamp in 64 bits.
 template <int DEG>
+__device__ __forceinline__ void preclamp64(const Coef<DEG>& c, v3a p, const float* cam, double* s) {
+    const double x = (double)p.x - cam[0], y = (double)p.y - cam[1], z = (double)p.z - cam[2];
+    const double n = x * x + y * y + z * z;
+    const double r = n > 0.0 ? 1.0 / sqrt(n) : 0.0;
+    double b[Coef<DEG>::N];
+    sh_values<DEG, double>(x * r, y * r, z * r, b);
+    c.template sum<double>(b, s);
+}
+
+// Colours of one Gaussian in every view; with MASK, which channels the clamp lets through (a
+// byte a view).  Rounding of the value before the clamp, in units of 2^-24: a direction is good to
+// 6, a basis value (slope at most 4.9) to 37, the sum of 16 products to 53 of the coefficients'
+// sum; nearer to zero than 64 the sign is taken from 64 bits, so that no gradient hangs on a
+// rounding.
+template <int DEG, bool MASK>
 __device__ __forceinline__ void write_colors(const ShArgs& a, int i, v3a p, const Coef<DEG>& c,
-                                             float* __restrict__ colors) {
+                                             float* __restrict__ colors, uint8_t* __restrict__ mask) {
+    float near[3] = {0.5f, 0.5f, 0.5f};
+    if constexpr (MASK) {
+#pragma unroll
+        for (int k = 0; k < Coef<DEG>::N; ++k)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) near[j] += fabsf(c.q[3 * k + j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) near[j] *= 0x1p-18f;
     for (int v = 0; v < a.V; ++v) {
-        float x = p.x - a.campos[3 * v], y = p.y - a.campos[3 * v + 1], z = p.z - a.campos[3 * v + 2];
+        const float* cam = a.campos + 3 * v;
+        float x = p.x - cam[0], y = p.y - cam[1], z = p.z - cam[2];
         normalize3(x, y, z);
         float b[Coef<DEG>::N], s[3];
         sh_values<DEG, float>(x, y, z, b);
         c.sum(b, s);
+        if constexpr (MASK) {
+            bool on[3], close = false;
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+                on[j] = s[j] >= 0.0f;
+                close |= fabsf(s[j]) < near[j];
+            }
+            if (close) {
+                double t[3];
+                preclamp64<DEG>(c, p, cam, t);
+#pragma unroll
+                for (int j = 0; j < 3; ++j) on[j] = t[j] >= 0.0;
+            }
+            mask[(long long)v * a.P + i] = (uint8_t)(on[0] | on[1] << 1 | on[2] << 2);
+        }
 #pragma unroll
         for (int j = 0; j < 3; ++j) s[j] = s[j] < 0.0f ? 0.0f : s[j];  // keeps a NaN
         store3(colors + ((long long)v * a.P + i) * 3, s[0], s[1], s[2]);
@@ -299,14 +368,15 @@ __device__ __forceinline__ void write_colors(const ShArgs& a, int i, v3a p, cons
 
 // One thread per Gaussian, its coefficients in registers for all views.  Bound by memory with
 // one view (62 bytes a Gaussian at degree 3), by the vector units with many.
-template <int DEG>
-__global__ void __launch_bounds__(CP_THREADS) k_sh_colors(ShArgs a, float* __restrict__ colors) {
+template <int DEG, bool MASK>
+__global__ void __launch_bounds__(CP_THREADS) k_sh_colors(ShArgs a, float* __restrict__ colors,
+                                                          uint8_t* __restrict__ mask) {
     const int i = blockIdx.x * CP_THREADS + threadIdx.x;
     if (i >= a.P) return;
     const v3a p = load3(a.xyz + 3LL * i);
     Coef<DEG> c;
     c.load(i, a);
-    write_colors<DEG>(a, i, p, c, colors);
+    write_colors<DEG, MASK>(a, i, p, c, colors, mask);
 }
 
 // ---- rows of features through LDS ------------------------------------------------
@@ -374,6 +444,7 @@ template <int DEG>
 __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, const float* __restrict__ features,
                                                                    uint32_t* __restrict__ codes,
                                                                    uint8_t* __restrict__ scales,
+                                                                   uint8_t* __restrict__ mask,
                                                                    float* __restrict__ colors) {
     using C = Coef<DEG>;
     __shared__ float4 s_rows[CP_THREADS / 64][ROWS_LDS / 4];
@@ -428,24 +499,16 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, con
     for (int j = 0; j < C::WORDS; ++j) codes[(long long)i * a.pitch + j] = w[j];
 #pragma unroll
     for (int b = 0; b < C::BLOCKS; ++b) scales[(long long)i * a.nb + b] = (uint8_t)(bytes >> (8 * b));
-    write_colors<DEG>(a, i, p, c, colors);
+    write_colors<DEG, true>(a, i, p, c, colors, mask);
 }
 
-// The value before the clamp in 64 bits.
-template <int DEG>
-__device__ __forceinline__ void preclamp64(const Coef<DEG>& c, v3a p, const float* cam, double* s) {
-    const double x = (double)p.x - cam[0], y = (double)p.y - cam[1], z = (double)p.z - cam[2];
-    const double n = x * x + y * y + z * z;
-    const double r = n > 0.0 ? 1.0 / sqrt(n) : 0.0;
-    double b[Coef<DEG>::N];
-    sh_values<DEG, double>(x * r, y * r, z * r, b);
-    c.template sum<double>(b, s);
-}
-
-// One thread per Gaussian, all views; the features' gradient rows leave through LDS.
+// One thread per Gaussian, all views; the features' gradient rows leave through LDS.  Which
+// channels take part comes from the forward's mask, so the constant coefficients (whose basis value
+// has no slope) are not read.
 // WANT_F: dfeatures is wanted (else at most its first coefficient, ddc).
 template <int DEG, bool WANT_F>
-__global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, const float* __restrict__ dcolors,
+__global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, const uint8_t* __restrict__ mask,
+                                                                   const float* __restrict__ dcolors,
                                                                    float* __restrict__ dxyz, float* __restrict__ ddc,
                                                                    float* __restrict__ dfeatures) {
     constexpr int N = Coef<DEG>::N, NF = WANT_F ? N : 1;
@@ -457,16 +520,6 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, con
     const v3a p = load3(a.xyz + 3LL * i);
     Coef<DEG> c;
     c.load(i, a);
-    // Rounding of the value before the clamp, in units of 2^-24: a direction is good to 6, a basis
-    // value (slope at most 4.9) to 37, the sum of 16 products to 53 of the coefficients' sum; nearer to
-    // zero than 64 the sign is taken from 64 bits, so that no gradient hangs on a rounding.
-    float near[3] = {0.5f, 0.5f, 0.5f};
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-#pragma unroll
-        for (int j = 0; j < 3; ++j) near[j] += fabsf(c.q[3 * k + j]);
-#pragma unroll
-    for (int j = 0; j < 3; ++j) near[j] *= 0x1p-18f;
     float acc[3 * NF];
 #pragma unroll
     for (int k = 0; k < 3 * NF; ++k) acc[k] = 0.0f;
@@ -474,38 +527,26 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, con
     for (int v = 0; v < a.V; ++v) {
         const float* cam = a.campos + 3 * v;
         const v3a gp = load3(dcolors + ((long long)v * a.P + i) * 3);
+        const uint32_t on = mask[(long long)v * a.P + i];
         float x = p.x - cam[0], y = p.y - cam[1], z = p.z - cam[2];
         const float r = normalize3(x, y, z);
-        float b[N], s[3];
+        float b[N];
         sh_values<DEG, float>(x, y, z, b);
-        c.sum(b, s);
-        bool on[3];
-        bool close = false;
-#pragma unroll
-        for (int j = 0; j < 3; ++j) {
-            on[j] = s[j] >= 0.0f;
-            close |= fabsf(s[j]) < near[j];
-        }
-        if (close) {
-            double t[3];
-            preclamp64<DEG>(c, p, cam, t);
-#pragma unroll
-            for (int j = 0; j < 3; ++j) on[j] = t[j] >= 0.0;
-        }
-        const float g[3] = {on[0] ? gp.x : 0.0f, on[1] ? gp.y : 0.0f, on[2] ? gp.z : 0.0f};
+        const float g[3] = {on & 1u ? gp.x : 0.0f, on & 2u ? gp.y : 0.0f, on & 4u ? gp.z : 0.0f};
 #pragma unroll
         for (int k = 0; k < NF; ++k)
 #pragma unroll
-            for (int j = 0; j < 3; ++j) acc[3 * k + j] += b[k] * g[j];
+            for (int j = 0; j < 3; ++j) acc[3 * k + j] = mad(b[k], g[j], acc[3 * k + j]);
         if (DEG > 0 && dxyz) {
             float w[N], gx, gy, gz;
 #pragma unroll
-            for (int k = 0; k < N; ++k) w[k] = c.q[3 * k] * g[0] + c.q[3 * k + 1] * g[1] + c.q[3 * k + 2] * g[2];
+            for (int k = 1; k < N; ++k)
+                w[k] = mad(c.q[3 * k], g[0], mad(c.q[3 * k + 1], g[1], c.q[3 * k + 2] * g[2]));
             sh_grad<DEG>(x, y, z, w, gx, gy, gz);
-            const float along = gx * x + gy * y + gz * z;
-            ax += r * (gx - along * x);
-            ay += r * (gy - along * y);
-            az += r * (gz - along * z);
+            const float along = mad(gx, x, mad(gy, y, gz * z));
+            ax = mad(r, mad(-along, x, gx), ax);
+            ay = mad(r, mad(-along, y, gy), ay);
+            az = mad(r, mad(-along, z, gz), az);
         }
     }
     if (first + lane < a.P) {
@@ -533,7 +574,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_accumulate_weights(int P, const 
                                                                    long long stride, float decay,
                                                                    float* __restrict__ acc) {
     const int i = blockIdx.x * CP_THREADS + threadIdx.x;
-    if (i < P) acc[i] = decay * acc[i] + w[i * stride];
+    if (i < P) acc[i] = mad(decay, acc[i], w[i * stride]);
 }
 
 // -------------------------------------------------------------------- eviction --
@@ -876,49 +917,52 @@ GSR_API int gsr_mx4_dequantize(long long R, int K, const uint32_t* codes, const 
 
 GSR_API int gsr_sh_colors(int P, int V, int degree, int M, const float* xyz, const float* dc, long long dc_stride,
                           const uint32_t* codes, const uint8_t* scales, const float* campos, float* colors,
-                          void* stream) {
+                          uint8_t* mask, void* stream) {
     if (int rc = check_colors(P, V, degree, M, xyz, dc, codes, scales, campos)) return rc;
     if (P == 0) return 0;
     if (!colors) return set_error("[gsr] gsr_sh_colors: null buffer");
     const ShArgs a = sh_args(P, V, M, xyz, dc, dc_stride, codes, scales, campos);
     const unsigned grid = grid_for(P, 1LL << 31);
     hipStream_t st = (hipStream_t)stream;
-    if (degree == 0) k_sh_colors<0><<<grid, CP_THREADS, 0, st>>>(a, colors);
-    else if (degree == 1) k_sh_colors<1><<<grid, CP_THREADS, 0, st>>>(a, colors);
-    else if (degree == 2) k_sh_colors<2><<<grid, CP_THREADS, 0, st>>>(a, colors);
-    else k_sh_colors<3><<<grid, CP_THREADS, 0, st>>>(a, colors);
+#define GSR_SH_COLORS(D)                                                                  \
+    if (mask) k_sh_colors<D, true><<<grid, CP_THREADS, 0, st>>>(a, colors, mask);         \
+    else k_sh_colors<D, false><<<grid, CP_THREADS, 0, st>>>(a, colors, nullptr)
+    if (degree == 0) { GSR_SH_COLORS(0); }
+    else if (degree == 1) { GSR_SH_COLORS(1); }
+    else if (degree == 2) { GSR_SH_COLORS(2); }
+    else { GSR_SH_COLORS(3); }
+#undef GSR_SH_COLORS
     return launched("sh_colors");
 }
 
 GSR_API int gsr_sh_colors_quantize(int P, int V, int degree, int M, const float* xyz, const float* features,
-                                   const float* campos, uint32_t* codes, uint8_t* scales, float* colors,
-                                   void* stream) {
+                                   const float* campos, uint32_t* codes, uint8_t* scales, uint8_t* mask,
+                                   float* colors, void* stream) {
     if (int rc = check_colors(P, V, degree, M, xyz, features, codes, scales, campos)) return rc;
     if (P == 0) return 0;
-    if (!colors) return set_error("[gsr] gsr_sh_colors_quantize: null buffer");
+    if (!mask || !colors) return set_error("[gsr] gsr_sh_colors_quantize: null buffer");
     const ShArgs a = sh_args(P, V, M, xyz, nullptr, 0, nullptr, nullptr, campos);
     const unsigned grid = grid_for(P, 1LL << 31);
     hipStream_t st = (hipStream_t)stream;
-    if (degree == 0) k_sh_colors_quantize<0><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, colors);
-    else if (degree == 1) k_sh_colors_quantize<1><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, colors);
-    else if (degree == 2) k_sh_colors_quantize<2><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, colors);
-    else k_sh_colors_quantize<3><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, colors);
+    if (degree == 0) k_sh_colors_quantize<0><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors);
+    else if (degree == 1) k_sh_colors_quantize<1><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors);
+    else if (degree == 2) k_sh_colors_quantize<2><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors);
+    else k_sh_colors_quantize<3><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors);
     return launched("sh_colors_quantize");
 }
 
-GSR_API int gsr_sh_colors_backward(int P, int V, int degree, int M, const float* xyz, const float* dc,
-                                   long long dc_stride, const uint32_t* codes, const uint8_t* scales,
-                                   const float* campos, const float* dcolors, float* dxyz, float* ddc,
-                                   float* dfeatures, void* stream) {
-    if (int rc = check_colors(P, V, degree, M, xyz, dc, codes, scales, campos)) return rc;
+GSR_API int gsr_sh_colors_backward(int P, int V, int degree, int M, const float* xyz, const uint32_t* codes,
+                                   const uint8_t* scales, const float* campos, const uint8_t* mask,
+                                   const float* dcolors, float* dxyz, float* ddc, float* dfeatures, void* stream) {
+    if (int rc = check_colors(P, V, degree, M, xyz, xyz, codes, scales, campos)) return rc;
     if (P == 0 || (!dxyz && !ddc && !dfeatures)) return 0;
-    if (!dcolors) return set_error("[gsr] gsr_sh_colors_backward: null buffer");
-    const ShArgs a = sh_args(P, V, M, xyz, dc, dc_stride, codes, scales, campos);
+    if (!mask || !dcolors) return set_error("[gsr] gsr_sh_colors_backward: null buffer");
+    const ShArgs a = sh_args(P, V, M, xyz, nullptr, 0, codes, scales, campos);
     const unsigned grid = grid_for(P, 1LL << 31);
     hipStream_t st = (hipStream_t)stream;
 #define GSR_SH_BACKWARD(D)                                                                              \
-    if (dfeatures) k_sh_colors_backward<D, true><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures); \
-    else k_sh_colors_backward<D, false><<<grid, CP_THREADS, 0, st>>>(a, dcolors, dxyz, ddc, dfeatures)
+    if (dfeatures) k_sh_colors_backward<D, true><<<grid, CP_THREADS, 0, st>>>(a, mask, dcolors, dxyz, ddc, dfeatures); \
+    else k_sh_colors_backward<D, false><<<grid, CP_THREADS, 0, st>>>(a, mask, dcolors, dxyz, ddc, dfeatures)
     if (degree == 0) { GSR_SH_BACKWARD(0); }
     else if (degree == 1) { GSR_SH_BACKWARD(1); }
     else if (degree == 2) { GSR_SH_BACKWARD(2); }

@@ -41,9 +41,9 @@ class _Rows(ctypes.Structure):
 
 for _name, _args in (("gsr_mx4_quantize", [_ll, _i, _vp, _ll, _vp, _vp, _vp]),
                      ("gsr_mx4_dequantize", [_ll, _i, _vp, _vp, _vp, _vp]),
-                     ("gsr_sh_colors", [_i, _i, _i, _i, _vp, _vp, _ll, _vp, _vp, _vp, _vp, _vp]),
-                     ("gsr_sh_colors_quantize", [_i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
-                     ("gsr_sh_colors_backward", [_i, _i, _i, _i, _vp, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+                     ("gsr_sh_colors", [_i, _i, _i, _i, _vp, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp]),
+                     ("gsr_sh_colors_quantize", [_i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+                     ("gsr_sh_colors_backward", [_i, _i, _i, _i] + [_vp] * 10),
                      ("gsr_accumulate_weights", [_i, _vp, _ll, _f, _vp, _vp]),
                      ("gsr_keep_heaviest", [_i, _vp, _i, ctypes.POINTER(_Group), _vp, _vp, _vp]),
                      ("gsr_take_rows", [_i, _vp, _i, ctypes.POINTER(_Rows), _vp])):
@@ -162,29 +162,54 @@ def _sh_check(what, xyz, campos, degree, M):
                            f"(degree {degree}, {M} coefficients)")
 
 
+def _buffers(xyz, V, single, grad):
+    """(colors [V, P, 3] or [P, 3], mask [V, P] for the backward or None)."""
+    P, dev = xyz.shape[0], xyz.device
+    colors = torch.empty((P, 3) if single else (V, P, 3), dtype=torch.float32, device=dev)
+    return colors, torch.empty((V, P), dtype=torch.uint8, device=dev) if grad else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _backward(g, saved, degree, M, dxyz, ddc, dfeatures):
+    xyz, campos, codes, scales, mask = saved
+    P = xyz.shape[0]
+    if P:
+        g = g.contiguous()
+        _call(xyz.device, _lib.gsr_sh_colors_backward, P, campos.shape[0], degree, M, xyz.data_ptr(), codes.data_ptr(),
+              scales.data_ptr(), campos.data_ptr(), mask.data_ptr(), g.data_ptr(), _ptr(dxyz), _ptr(ddc),
+              _ptr(dfeatures))
+
+
 class _ShColors(torch.autograd.Function):
     """colors [V, P, 3] ([P, 3] with `single`) from xyz, the constant coefficients dc [P, 3] and codes."""
 
     @staticmethod
     def forward(ctx, xyz, dc, campos, codes, scales, degree, M, single):
-        colors = _forward(xyz, dc, campos, codes, scales, degree, M, single)
-        ctx.save_for_backward(xyz, dc, campos, codes, scales)
+        P, V = xyz.shape[0], campos.shape[0]
+        colors, mask = _buffers(xyz, V, single, any(ctx.needs_input_grad))
+        if P:
+            _call(xyz.device, _lib.gsr_sh_colors, P, V, degree, M, xyz.data_ptr(), dc.data_ptr(), dc.stride(0),
+                  codes.data_ptr(), scales.data_ptr(), campos.data_ptr(), colors.data_ptr(), _ptr(mask))
+        ctx.save_for_backward(xyz, campos, codes, scales, mask)
         ctx.degree, ctx.M = degree, M
         return colors
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        xyz, dc, campos, codes, scales = ctx.saved_tensors
+        xyz = ctx.saved_tensors[0]
         dxyz = torch.empty_like(xyz) if ctx.needs_input_grad[0] else None
-        ddc = torch.empty((xyz.shape[0], 3), dtype=torch.float32, device=xyz.device) if ctx.needs_input_grad[1] else None
-        _backward(g, xyz, dc, campos, codes, scales, ctx.degree, ctx.M, dxyz, ddc, None)
+        ddc = torch.empty_like(xyz) if ctx.needs_input_grad[1] else None
+        _backward(g, ctx.saved_tensors, ctx.degree, ctx.M, dxyz, ddc, None)
         return dxyz, ddc, None, None, None, None, None, None
 
 
 class _ShColorsQuantized(torch.autograd.Function):
-    """colors [V, P, 3] ([P, 3] with `single`) from xyz and fp32 features [P, M, 3]; the
-    backward reads the codes of the forward and, of the features, the constant coefficients."""
+    """colors [V, P, 3] ([P, 3] with `single`) from xyz and fp32 features [P, M, 3]; what is kept
+    of the features for the backward are their codes, 26 bytes a Gaussian, and a byte a view."""
 
     @staticmethod
     def forward(ctx, xyz, features, campos, degree, single):
@@ -192,46 +217,24 @@ class _ShColorsQuantized(torch.autograd.Function):
         K, V, dev = 3 * (M - 1), campos.shape[0], xyz.device
         codes = torch.empty((P, 4 * _words(K)), dtype=torch.uint8, device=dev)
         scales = torch.empty((P, _blocks(K)), dtype=torch.uint8, device=dev)
-        colors = torch.empty((P, 3) if single else (V, P, 3), dtype=torch.float32, device=dev)
+        colors, mask = _buffers(xyz, V, single, True)
         if P:
             _call(dev, _lib.gsr_sh_colors_quantize, P, V, degree, M, xyz.data_ptr(), features.data_ptr(),
-                  campos.data_ptr(), codes.data_ptr(), scales.data_ptr(), colors.data_ptr())
-        ctx.save_for_backward(xyz, features, campos, codes, scales)
+                  campos.data_ptr(), codes.data_ptr(), scales.data_ptr(), mask.data_ptr(), colors.data_ptr())
+        ctx.save_for_backward(xyz, campos, codes, scales, mask)
         ctx.degree, ctx.M = degree, M
         return colors
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        xyz, features, campos, codes, scales = ctx.saved_tensors
+        xyz = ctx.saved_tensors[0]
         dxyz = torch.empty_like(xyz) if ctx.needs_input_grad[0] else None
         df = None
         if ctx.needs_input_grad[1]:
             df = torch.empty((xyz.shape[0], ctx.M, 3), dtype=torch.float32, device=xyz.device)
-        _backward(g, xyz, features[:, 0], campos, codes, scales, ctx.degree, ctx.M, dxyz, None, df)
+        _backward(g, ctx.saved_tensors, ctx.degree, ctx.M, dxyz, None, df)
         return dxyz, df, None, None, None
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _forward(xyz, dc, campos, codes, scales, degree, M, single):
-    P, V = xyz.shape[0], campos.shape[0]
-    colors = torch.empty((P, 3) if single else (V, P, 3), dtype=torch.float32, device=xyz.device)
-    if P:
-        _call(xyz.device, _lib.gsr_sh_colors, P, V, degree, M, xyz.data_ptr(), dc.data_ptr(), dc.stride(0),
-              codes.data_ptr(), scales.data_ptr(), campos.data_ptr(), colors.data_ptr())
-    return colors
-
-
-def _backward(g, xyz, dc, campos, codes, scales, degree, M, dxyz, ddc, dfeatures):
-    P = xyz.shape[0]
-    if P:
-        g = g.contiguous()
-        _call(xyz.device, _lib.gsr_sh_colors_backward, P, campos.shape[0], degree, M, xyz.data_ptr(), dc.data_ptr(),
-              dc.stride(0), codes.data_ptr(), scales.data_ptr(), campos.data_ptr(), g.data_ptr(), _ptr(dxyz),
-              _ptr(ddc), _ptr(dfeatures))
 
 
 def sh_colors(xyz, features_dc, rest, campos, degree):

@@ -39,28 +39,29 @@ GSR_API int gsr_mx4_dequantize(long long R, int K, const uint32_t* codes, const 
 /* Colours of P Gaussians from V camera positions (utils/sh_utils.py:57-112 eval_sh, + 0.5 and
  * clamp as forward.cu:20-71), colors [V, P, 3]:
  *   u = xyz - campos[v], d = u / |u| (0 where u is 0);
- *   colors = max(0, 0.5 + Y_0 dc + sum_{1 <= k < (degree+1)^2} Y_k(d) rest_k).
+ *   p = 0.5 + Y_0 dc + sum_{1 <= k < (degree+1)^2} Y_k(d) rest_k;  colors = max(0, p).
  * dc: row i at dc + i * dc_stride (3 floats); codes / scales: rows of 3 (M - 1) floats
  * (coefficient-major, as the arena's features block).  0 <= degree <= 3,
- * (degree + 1)^2 <= M <= 16, 1 <= V <= GSR_MAX_VIEWS; campos: device [V, 3]. */
+ * (degree + 1)^2 <= M <= 16, 1 <= V <= GSR_MAX_VIEWS; campos: device [V, 3].  mask [V, P],
+ * for the backward, or NULL: bit c of a byte is set where channel c has p >= 0 (decided in
+ * 64 bits where 32 cannot). */
 GSR_API int gsr_sh_colors(int P, int V, int degree, int M, const float* xyz, const float* dc, long long dc_stride,
                           const uint32_t* codes, const uint8_t* scales, const float* campos, float* colors,
-                          void* stream);
+                          uint8_t* mask, void* stream);
 /* The same from fp32 features [P, M, 3] whose coefficients above the constant one are rounded
  * in the call.  codes / scales: rows of 3 (M - 1) values as gsr_mx4_quantize writes them, of which
- * those that `degree` reads are written (for gsr_sh_colors_backward of the same degree). */
+ * those that `degree` reads are written; with mask what gsr_sh_colors_backward of the same
+ * degree reads. */
 GSR_API int gsr_sh_colors_quantize(int P, int V, int degree, int M, const float* xyz, const float* features,
-                                   const float* campos, uint32_t* codes, uint8_t* scales, float* colors,
-                                   void* stream);
-/* Gradients for dcolors [V, P, 3], summed over the views in order; a colour channel
- * takes part where its value before the clamp is >= 0 (the sign is decided in 64
- * bits where 32 cannot).  Each of the outputs may be NULL: dxyz [P, 3] (0 where u is 0);
- * ddc [P, 3]; dfeatures [P, M, 3], coefficient 0 = d/d(dc), the others the gradient of
- * the decoded value (straight through the rounding), 0 above the degree. */
-GSR_API int gsr_sh_colors_backward(int P, int V, int degree, int M, const float* xyz, const float* dc,
-                                   long long dc_stride, const uint32_t* codes, const uint8_t* scales,
-                                   const float* campos, const float* dcolors, float* dxyz, float* ddc,
-                                   float* dfeatures, void* stream);
+                                   const float* campos, uint32_t* codes, uint8_t* scales, uint8_t* mask,
+                                   float* colors, void* stream);
+/* Gradients for dcolors [V, P, 3], summed over the views in order; a channel takes part
+ * where the forward's mask has its bit.  Each of the outputs may be NULL: dxyz [P, 3] (0 where
+ * u is 0); ddc [P, 3]; dfeatures [P, M, 3], coefficient 0 = d/d(dc), the others the gradient
+ * of the decoded value (straight through the rounding), 0 above the degree. */
+GSR_API int gsr_sh_colors_backward(int P, int V, int degree, int M, const float* xyz, const uint32_t* codes,
+                                   const uint8_t* scales, const float* campos, const uint8_t* mask,
+                                   const float* dcolors, float* dxyz, float* ddc, float* dfeatures, void* stream);
 
 /* acc[i] <- decay * acc[i] + weights[i * stride], i < P (accumulated blend weights). */
 GSR_API int gsr_accumulate_weights(int P, const float* weights, long long stride, float decay, float* acc,

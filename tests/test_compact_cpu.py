@@ -33,12 +33,14 @@ def test_c_calls_validate_without_the_device():
     assert L.gsr_mx4_quantize(0, 45, None, 45, None, None, None) == 0
     assert L.gsr_mx4_quantize(5, 0, None, 0, None, None, None) == 0
     assert L.gsr_mx4_dequantize(3, 45, 16, None, 16, None) != 0 and "null buffer" in err()
-    assert L.gsr_sh_colors(0, 1, 3, 16, None, None, 3, None, None, None, None, None) == 0
+    assert L.gsr_sh_colors(0, 1, 3, 16, None, None, 3, None, None, None, None, None, None) == 0
     for V, deg, M in ((0, 0, 1), (17, 0, 1), (1, 4, 25), (1, 3, 15), (1, -1, 1), (1, 0, 17)):
-        assert L.gsr_sh_colors(4, V, deg, M, 16, 16, 3, 16, 16, 16, 16, None) != 0
-    assert L.gsr_sh_colors(4, 1, 1, 4, 16, 16, 3, None, 16, 16, 16, None) != 0 and "null buffer" in err()
-    assert L.gsr_sh_colors_backward(4, 1, 1, 4, 16, 16, 3, 16, 16, 16, None, 16, None, None, None) != 0
-    assert L.gsr_sh_colors_backward(4, 1, 1, 4, 16, 16, 3, 16, 16, 16, None, None, None, None, None) == 0
+        assert L.gsr_sh_colors(4, V, deg, M, 16, 16, 3, 16, 16, 16, 16, None, None) != 0
+    assert L.gsr_sh_colors(4, 1, 1, 4, 16, 16, 3, None, 16, 16, 16, None, None) != 0 and "null buffer" in err()
+    assert L.gsr_sh_colors_backward(4, 1, 1, 4, 16, 16, 16, 16, 16, None, 16, None, None, None) != 0
+    assert L.gsr_sh_colors_backward(4, 1, 1, 4, 16, 16, 16, 16, None, 16, 16, None, None, None) != 0 and "null" in err()
+    assert L.gsr_sh_colors_quantize(4, 1, 1, 4, 16, 16, 16, 16, 16, None, 16, None) != 0 and "null buffer" in err()
+    assert L.gsr_sh_colors_backward(4, 1, 1, 4, 16, 16, 16, 16, None, None, None, None, None, None) == 0
     assert L.gsr_accumulate_weights(4, None, 1, 1.0, 16, None) != 0
 
     def groups(*g):
