@@ -581,10 +581,14 @@ __global__ void __launch_bounds__(CP_THREADS) k_accumulate_weights(int P, const 
 // The rows to keep of a group are its last `recent` ones and the heaviest `pick` of those
 // before them.  Radix selection: three histogram passes (11, 11, 10 bits from the top) find the
 // key T of the pick-th heaviest row and how many of the rows equal to it are kept (`ties`, the
-// lowest first); a count and a write pass then put the ids in order.  Every count is an
-// integer, so the result does not depend on the order of the atomics.
+// lowest first); then the ids are written in order.  Every count is an integer, so the result
+// does not depend on the order of the atomics.
+//   One block per group does it all for groups of up to KEEP_SMALL rows, the keys in registers;
+// larger groups take a launch per pass over tiles of KEEP_TILE rows: what is read, 4 bytes a row
+// and pass from the caches, is less than what the launches and their dependences cost.
 constexpr int KEEP_TILE = CP_THREADS * 16;  // rows per block
 constexpr int KEEP_BINS = 2048;
+constexpr int KEEP_SMALL_THREADS = 1024, KEEP_SMALL = KEEP_SMALL_THREADS * 16;
 
 struct KeepGroup {
     int begin, end, old_end;  // rows [begin, old_end) compete, [old_end, end) are kept
@@ -675,6 +679,99 @@ __device__ __forceinline__ KeepSel find_bin(const uint32_t* hist, uint32_t need,
     return *s_out;
 }
 
+// Counts digit d of the active lanes; lanes that share one digit (equal weights) add as one.
+__device__ __forceinline__ void keep_add(uint32_t* h, uint32_t d, bool in) {
+    const unsigned long long act = __ballot(in);
+    if (act == 0) return;
+    const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)d, __builtin_ctzll(act));
+    if (__ballot(in && d == d0) == act) {
+        if ((threadIdx.x & 63) == 0) atomicAdd(&h[d0], (uint32_t)__popcll(act));
+    } else if (in) {
+        atomicAdd(&h[d], 1u);
+    }
+}
+
+// Keys [i, i + 16) of rows below `end` (0 behind it).
+__device__ __forceinline__ void keep_load16(const float* __restrict__ w, long long i, long long end, uint32_t (&key)[16]) {
+    v4a v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        v[q] = v4a{0.0f, 0.0f, 0.0f, 0.0f};
+        if (i + 4 * q + 4 <= end) {
+            v[q] = *reinterpret_cast<const v4a*>(w + i + 4 * q);
+        } else {
+            if (i + 4 * q < end) v[q].x = w[i + 4 * q];
+            if (i + 4 * q + 1 < end) v[q].y = w[i + 4 * q + 1];
+            if (i + 4 * q + 2 < end) v[q].z = w[i + 4 * q + 2];
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        key[4 * q] = keep_key(v[q].x); key[4 * q + 1] = keep_key(v[q].y);
+        key[4 * q + 2] = keep_key(v[q].z); key[4 * q + 3] = keep_key(v[q].w);
+    }
+}
+
+template <int PASS>
+__device__ __forceinline__ bool keep_digit(uint32_t key, uint32_t prefix, uint32_t& d) {
+    d = PASS == 0 ? key >> 21 : PASS == 1 ? (key >> 10) & 2047u : key & 1023u;
+    return PASS == 0 || (PASS == 1 ? key >> 21 : key >> 10) == prefix;
+}
+
+// One pass over the keys of a small group: the digits found before it -> one more.
+template <int PASS>
+__device__ __forceinline__ KeepSel keep_small_pass(const uint32_t (&key)[16], int n, KeepSel st, uint32_t* h,
+                                                   uint32_t* s_wave, KeepSel* s_out) {
+    __syncthreads();
+    for (int k = threadIdx.x; k < KEEP_BINS; k += KEEP_SMALL_THREADS) h[k] = 0u;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        uint32_t d;
+        const bool in = keep_digit<PASS>(key[k], st.prefix, d) && (int)threadIdx.x * 16 + k < n;
+        keep_add(h, d, in);
+    }
+    __syncthreads();
+    const KeepSel b = find_bin<KEEP_SMALL_THREADS>(h, st.need, s_wave, s_out);
+    return {(st.prefix << (PASS == 2 ? 10 : 11)) | b.prefix, b.need};
+}
+
+__global__ void __launch_bounds__(KEEP_SMALL_THREADS) k_keep_small(KeepArgs a, const float* __restrict__ w,
+                                                                   int* __restrict__ ids) {
+    __shared__ uint32_t h[KEEP_BINS];
+    __shared__ uint32_t s_wave[KEEP_SMALL_THREADS / 64];
+    __shared__ KeepSel s_out;
+    const KeepGroup G = a.g[blockIdx.x];
+    const int n = G.old_end - G.begin, first = threadIdx.x * 16;
+    if (G.pick > 0) {  // the whole block
+        uint32_t key[16];
+        keep_load16(w, (long long)G.begin + first, G.old_end, key);
+        KeepSel st = {0u, (uint32_t)G.pick};
+        st = keep_small_pass<0>(key, n, st, h, s_wave, &s_out);
+        st = keep_small_pass<1>(key, n, st, h, s_wave, &s_out);
+        st = keep_small_pass<2>(key, n, st, h, s_wave, &s_out);
+        uint32_t gt = 0, eq = 0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            gt += first + k < n && key[k] > st.prefix;
+            eq += first + k < n && key[k] == st.prefix;
+        }
+        const uint32_t before = block_scan_excl<KEEP_SMALL_THREADS>(gt | eq << 16, s_wave);  // at most 16384 each
+        gt = before & 0xFFFFu;
+        eq = before >> 16;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            if (first + k < n) {
+                const bool up = key[k] > st.prefix, tie = key[k] == st.prefix;
+                if (up || (tie && eq < st.need)) ids[G.out + gt + (eq < st.need ? eq : st.need)] = G.begin + first + k;
+                gt += up;
+                eq += tie;
+            }
+        }
+    }
+    for (int i = G.old_end + threadIdx.x; i < G.end; i += KEEP_SMALL_THREADS) ids[G.out + G.pick + (i - G.old_end)] = i;
+}
+
 __global__ void __launch_bounds__(CP_THREADS) k_keep_clear(uint32_t* __restrict__ p, int n) {
     for (int i = blockIdx.x * CP_THREADS + threadIdx.x; i < n; i += gridDim.x * CP_THREADS) p[i] = 0u;
 }
@@ -701,19 +798,17 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_hist(KeepArgs a, KeepWs ws,
     const int tile = blockIdx.x, g = keep_group_of(a, tile);
     const KeepGroup G = a.g[g];
     if (G.pick == 0) return;  // nothing to look for (the whole block)
+    uint32_t key[16];
+    const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE + threadIdx.x * 16;
+    keep_load16(w, base, G.old_end, key);
     for (int k = threadIdx.x; k < KEEP_BINS; k += CP_THREADS) h[k] = 0u;
     const KeepSel st = keep_state<PASS>(a, ws, g, tile, s_wave, &s_out);
     __syncthreads();
-    const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE;
-#pragma unroll 4
+#pragma unroll
     for (int k = 0; k < 16; ++k) {
-        const long long i = base + k * CP_THREADS + threadIdx.x;
-        if (i < G.old_end) {
-            const uint32_t key = keep_key(w[i]);
-            const bool in = PASS == 0 || (PASS == 1 ? key >> 21 : key >> 10) == st.prefix;
-            const uint32_t d = PASS == 0 ? key >> 21 : PASS == 1 ? (key >> 10) & 2047u : key & 1023u;
-            if (in) atomicAdd(&h[d], 1u);
-        }
+        uint32_t d;
+        const bool in = keep_digit<PASS>(key[k], st.prefix, d) && base + k < G.old_end;
+        keep_add(h, d, in);
     }
     __syncthreads();
     uint32_t* out = ws.hist + ((size_t)g * 3 + PASS) * KEEP_BINS;
@@ -729,15 +824,14 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_count(KeepArgs a, KeepWs ws
     const KeepGroup G = a.g[g];
     uint32_t gt = 0, eq = 0;
     if (G.pick > 0) {
+        uint32_t key[16];
+        const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE + threadIdx.x * 16;
+        keep_load16(w, base, G.old_end, key);
         const uint32_t T = keep_state<3>(a, ws, g, tile, s_wave, &s_out).prefix;
-        const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE;
+#pragma unroll
         for (int k = 0; k < 16; ++k) {
-            const long long i = base + k * CP_THREADS + threadIdx.x;
-            if (i < G.old_end) {
-                const uint32_t key = keep_key(w[i]);
-                gt += key > T;
-                eq += key == T;
-            }
+            gt += base + k < G.old_end && key[k] > T;
+            eq += base + k < G.old_end && key[k] == T;
         }
     }
     const uint32_t both = gt | eq << 16;  // at most KEEP_TILE = 4096 of each
@@ -745,20 +839,21 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_count(KeepArgs a, KeepWs ws
     if (threadIdx.x == CP_THREADS - 1) ws.count[tile] = make_uint2((before + both) & 0xFFFFu, (before + both) >> 16);
 }
 
-// Thread t writes rows [16 t, 16 t + 16) of its tile: slot = first slot + kept rows before.
+// A tile's kept rows: ranked by a scan over the threads (16 rows each, in order), gathered in LDS
+// and written in one piece behind those of the tiles before.
 __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws, const float* __restrict__ w,
                                                            int* __restrict__ ids) {
     __shared__ uint32_t s_wave[CP_THREADS / 64];
     __shared__ unsigned long long s_sum;
+    __shared__ int s_ids[KEEP_TILE];
+    __shared__ uint32_t s_n;
     const int tile = blockIdx.x, g = keep_group_of(a, tile);
     const KeepGroup G = a.g[g];
-    const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE + threadIdx.x * 16;
-    uint32_t T = 0xFFFFFFFFu, ties = 0;  // no key reaches this T
-    uint32_t gt0 = 0, eq0 = 0;
-    if (G.pick > 0) {
+    const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE, first = base + threadIdx.x * 16;
+    if (G.pick > 0 && base < G.old_end) {  // the whole block
+        uint32_t key[16];
+        keep_load16(w, first, G.old_end, key);
         const KeepSel st = ws.sel[g * 3 + 2];
-        T = st.prefix;
-        ties = st.need;
         if (threadIdx.x == 0) s_sum = 0;
         __syncthreads();
         unsigned long long sum = 0;
@@ -767,33 +862,30 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
             sum += c.x | (unsigned long long)c.y << 32;
         }
         if (sum) atomicAdd(&s_sum, sum);
-        __syncthreads();
-        gt0 = (uint32_t)s_sum;
-        eq0 = (uint32_t)(s_sum >> 32);
-    }
-    uint32_t key[16], both = 0;
+        uint32_t both = 0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        key[k] = base + k < G.old_end ? keep_key(w[base + k]) : 0u;
-        const bool in = base + k < G.old_end;
-        both += (in && key[k] > T ? 1u : 0u) + (in && key[k] == T ? 1u << 16 : 0u);
-    }
-    const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave);
-    gt0 += before & 0xFFFFu;
-    eq0 += before >> 16;
+        for (int k = 0; k < 16; ++k)
+            if (first + k < G.old_end) both += key[k] > st.prefix ? 1u : key[k] == st.prefix ? 1u << 16 : 0u;
+        const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave);  // (its barriers also end the sum)
+        const uint32_t gt0 = (uint32_t)s_sum, eq0 = (uint32_t)(s_sum >> 32);
+        const uint32_t ties = eq0 < st.need ? st.need - eq0 : 0u;  // left for this tile
+        uint32_t gt = before & 0xFFFFu, eq = before >> 16;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        const long long i = base + k;
-        if (i >= G.end) break;
-        if (i >= G.old_end) {
-            ids[G.out + G.pick + (i - G.old_end)] = (int)i;
-            continue;
+        for (int k = 0; k < 16; ++k) {
+            if (first + k < G.old_end) {
+                const bool up = key[k] > st.prefix, tie = key[k] == st.prefix;
+                if (up || (tie && eq < ties)) s_ids[gt + (eq < ties ? eq : ties)] = (int)(first + k);
+                gt += up;
+                eq += tie;
+            }
         }
-        const bool up = key[k] > T, tie = key[k] == T;
-        if (up || (tie && eq0 < ties)) ids[G.out + gt0 + (eq0 < ties ? eq0 : ties)] = (int)i;
-        gt0 += up;
-        eq0 += tie;
+        if (threadIdx.x == CP_THREADS - 1) s_n = gt + (eq < ties ? eq : ties);
+        __syncthreads();
+        int* out = ids + G.out + gt0 + (eq0 < st.need ? eq0 : st.need);
+        for (uint32_t k = threadIdx.x; k < s_n; k += CP_THREADS) out[k] = s_ids[k];
     }
+    const long long lo = base > G.old_end ? base : G.old_end, hi = base + KEEP_TILE < G.end ? base + KEEP_TILE : G.end;
+    for (long long i = lo + threadIdx.x; i < hi; i += CP_THREADS) ids[G.out + G.pick + (i - G.old_end)] = (int)i;
 }
 
 // ------------------------------------------------------------------------ rows --
@@ -991,7 +1083,7 @@ GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const g
         return set_error("[gsr] gsr_keep_heaviest: at most " + std::to_string(GSR_KEEP_MAX_GROUPS) + " groups a call");
     if (n_groups > 0 && !groups) return set_error("[gsr] gsr_keep_heaviest: null groups");
     KeepArgs a{};
-    int last = 0;
+    int last = 0, most = 0;
     long long out = 0;
     for (int g = 0; g < n_groups; ++g) {
         const gsr_keep_group& q = groups[g];
@@ -1004,10 +1096,15 @@ GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const g
         a.g[a.n++] = {q.begin, q.end, q.end - q.recent, q.keep - q.recent, (int)out, a.tiles};
         a.tiles += (q.end - q.begin + KEEP_TILE - 1) / KEEP_TILE;
         out += q.keep;
+        most = std::max(most, q.end - q.begin);
     }
     if (a.n == 0) return 0;
     if (!weights || !ids || !ws) return set_error("[gsr] gsr_keep_heaviest: null buffer");
     hipStream_t st = (hipStream_t)stream;
+    if (most <= KEEP_SMALL) {
+        k_keep_small<<<a.n, KEEP_SMALL_THREADS, 0, st>>>(a, weights, ids);
+        return launched("keep_heaviest");
+    }
     const KeepWs w = keep_ws(ws);
     const int words = a.n * 3 * KEEP_BINS;
     k_keep_clear<<<grid_for(words, 1024), CP_THREADS, 0, st>>>(w.hist, words);
