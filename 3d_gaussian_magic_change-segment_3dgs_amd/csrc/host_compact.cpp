@@ -1,0 +1,251 @@
+// host_compact.cpp -- the host side of the compact-scene operators in C++ (part of the torch
+// extension "gsr_host"): allocation, the libgsr calls of include/gsr_compact.h and the autograd
+// functions, as gsr_train/compact.py does them over ctypes.  The Python layer checks the arguments of
+// the single operators before it calls in here (take_rows, whose tensors are many, is checked here);
+// a training step of colours costs ~90 us of host time less than through Python's autograd.
+#include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+
+#include <cstdint>
+#include <stdexcept>
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "gsr_compact.h"
+
+namespace {
+
+void check(int rc) {
+    if (rc) throw std::runtime_error(gsr_last_error());
+}
+void* cur_stream() { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
+using Guard = c10::hip::HIPGuardMasqueradingAsCUDA;
+
+int64_t words(int64_t K) { return (K + 7) / 8; }
+int64_t blocks(int64_t K) { return (K + GSR_MX_BLOCK - 1) / GSR_MX_BLOCK; }
+at::TensorOptions like(const at::Tensor& t, at::ScalarType type) {
+    return at::TensorOptions().dtype(type).device(t.device());
+}
+const uint32_t* code_ptr(const at::Tensor& t) { return reinterpret_cast<const uint32_t*>(t.data_ptr<uint8_t>()); }
+uint32_t* code_out(at::Tensor& t) { return reinterpret_cast<uint32_t*>(t.data_ptr<uint8_t>()); }
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> mx4_quantize(const at::Tensor& x) {
+    Guard guard(x.device());
+    const int64_t R = x.size(0), K = x.size(1);
+    at::Tensor codes = at::empty({R, 4 * words(K)}, like(x, at::kByte));
+    at::Tensor scales = at::empty({R, blocks(K)}, like(x, at::kByte));
+    if (R && K)
+        check(gsr_mx4_quantize(R, (int)K, x.data_ptr<float>(), x.stride(0), code_out(codes),
+                               scales.data_ptr<uint8_t>(), cur_stream()));
+    return {codes, scales};
+}
+
+at::Tensor mx4_dequantize(const at::Tensor& codes, const at::Tensor& scales, int64_t K) {
+    Guard guard(codes.device());
+    at::Tensor x = at::empty({codes.size(0), K}, like(codes, at::kFloat));
+    if (x.numel())
+        check(gsr_mx4_dequantize(codes.size(0), (int)K, code_ptr(codes), scales.data_ptr<uint8_t>(),
+                                 x.data_ptr<float>(), cur_stream()));
+    return x;
+}
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+at::Tensor colors_for(const at::Tensor& xyz, int64_t V, bool single) {
+    const int64_t P = xyz.size(0);
+    return single ? at::empty({P, 3}, like(xyz, at::kFloat)) : at::empty({V, P, 3}, like(xyz, at::kFloat));
+}
+
+at::Tensor colors_of(const at::Tensor& xyz, const at::Tensor& dc, const at::Tensor& campos, const at::Tensor& codes,
+                     const at::Tensor& scales, int64_t degree, int64_t M, bool single, at::Tensor* mask) {
+    const int64_t P = xyz.size(0), V = campos.size(0);
+    at::Tensor colors = colors_for(xyz, V, single);
+    if (mask) *mask = at::empty({V, P}, like(xyz, at::kByte));
+    if (P)
+        check(gsr_sh_colors((int)P, (int)V, (int)degree, (int)M, xyz.data_ptr<float>(), dc.data_ptr<float>(),
+                            dc.stride(0), code_ptr(codes), scales.data_ptr<uint8_t>(), campos.data_ptr<float>(),
+                            colors.data_ptr<float>(), mask ? mask->data_ptr<uint8_t>() : nullptr, cur_stream()));
+    return colors;
+}
+
+void keep(AutogradContext* ctx, const at::Tensor& xyz, const at::Tensor& campos, const at::Tensor& codes,
+          const at::Tensor& scales, const at::Tensor& mask, int64_t degree, int64_t M) {
+    ctx->save_for_backward({xyz, campos, codes, scales, mask});
+    ctx->saved_data["degree"] = degree;
+    ctx->saved_data["M"] = M;
+}
+
+// The gradients wanted of (dxyz, ddc or dfeatures); a second derivative is refused when it is taken.
+variable_list gradients(AutogradContext* ctx, const at::Tensor& g_in, bool features) {
+    const auto sv = ctx->get_saved_variables();
+    const at::Tensor &xyz = sv[0], &campos = sv[1], &codes = sv[2], &scales = sv[3], &mask = sv[4];
+    const int64_t P = xyz.size(0), M = ctx->saved_data["M"].toInt(), degree = ctx->saved_data["degree"].toInt();
+    Guard guard(xyz.device());
+    const bool twice = at::GradMode::is_enabled() && g_in.requires_grad();
+    variable_list out(2);
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const at::Tensor g = g_in.contiguous();
+        if (ctx->needs_input_grad(0)) out[0] = at::empty({P, 3}, like(xyz, at::kFloat));
+        if (ctx->needs_input_grad(1))
+            out[1] = features ? at::empty({P, M, 3}, like(xyz, at::kFloat)) : at::empty({P, 3}, like(xyz, at::kFloat));
+        float* second = out[1].defined() ? out[1].data_ptr<float>() : nullptr;
+        if (P)
+            check(gsr_sh_colors_backward((int)P, (int)campos.size(0), (int)degree, (int)M, xyz.data_ptr<float>(),
+                                         code_ptr(codes), scales.data_ptr<uint8_t>(), campos.data_ptr<float>(),
+                                         mask.data_ptr<uint8_t>(), g.data_ptr<float>(),
+                                         out[0].defined() ? out[0].data_ptr<float>() : nullptr,
+                                         features ? nullptr : second, features ? second : nullptr, cur_stream()));
+    }
+    if (twice) {
+        for (int k = 0; k < 2; ++k)
+            if (out[k].defined()) {
+                auto err = std::make_shared<torch::autograd::DelayedError>(
+                    "trying to differentiate twice a function that was marked with @once_differentiable", 1);
+                at::Tensor v = out[k].detach();
+                v.set_requires_grad(true);
+                out[k] = (*err)({v})[0];
+            }
+    }
+    return out;
+}
+
+struct ShColorsFn : public torch::autograd::Function<ShColorsFn> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& xyz, const at::Tensor& dc,
+                              const at::Tensor& campos, const at::Tensor& codes, const at::Tensor& scales,
+                              int64_t degree, int64_t M, bool single) {
+        at::Tensor mask;
+        at::Tensor colors = colors_of(xyz, dc, campos, codes, scales, degree, M, single, &mask);
+        keep(ctx, xyz, campos, codes, scales, mask, degree, M);
+        return colors;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list go) {
+        const variable_list g = gradients(ctx, go[0], false);
+        return {g[0], g[1], {}, {}, {}, {}, {}, {}};
+    }
+};
+
+at::Tensor quantized_of(const at::Tensor& xyz, const at::Tensor& features, const at::Tensor& campos, int64_t degree,
+                        bool single, at::Tensor& codes, at::Tensor& scales, at::Tensor& mask) {
+    const int64_t P = xyz.size(0), V = campos.size(0), M = features.size(1), K = 3 * (M - 1);
+    codes = at::empty({P, 4 * words(K)}, like(xyz, at::kByte));
+    scales = at::empty({P, blocks(K)}, like(xyz, at::kByte));
+    mask = at::empty({V, P}, like(xyz, at::kByte));
+    at::Tensor colors = colors_for(xyz, V, single);
+    if (P)
+        check(gsr_sh_colors_quantize((int)P, (int)V, (int)degree, (int)M, xyz.data_ptr<float>(),
+                                     features.data_ptr<float>(), campos.data_ptr<float>(), code_out(codes),
+                                     scales.data_ptr<uint8_t>(), mask.data_ptr<uint8_t>(), colors.data_ptr<float>(),
+                                     cur_stream()));
+    return colors;
+}
+
+struct ShColorsQuantizedFn : public torch::autograd::Function<ShColorsQuantizedFn> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& xyz, const at::Tensor& features,
+                              const at::Tensor& campos, int64_t degree, bool single) {
+        at::Tensor codes, scales, mask;
+        at::Tensor colors = quantized_of(xyz, features, campos, degree, single, codes, scales, mask);
+        keep(ctx, xyz, campos, codes, scales, mask, degree, features.size(1));
+        return colors;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list go) {
+        const variable_list g = gradients(ctx, go[0], true);
+        return {g[0], g[1], {}, {}, {}};
+    }
+};
+
+bool wanted(const at::Tensor& a, const at::Tensor& b) {
+    return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad());
+}
+
+}  // namespace
+
+at::Tensor sh_colors(const at::Tensor& xyz, const at::Tensor& dc, const at::Tensor& campos, const at::Tensor& codes,
+                     const at::Tensor& scales, int64_t degree, int64_t M, bool single) {
+    Guard guard(xyz.device());
+    if (wanted(xyz, dc)) return ShColorsFn::apply(xyz, dc, campos, codes, scales, degree, M, single);
+    return colors_of(xyz, dc, campos, codes, scales, degree, M, single, nullptr);
+}
+
+at::Tensor sh_colors_quantized(const at::Tensor& xyz, const at::Tensor& features, const at::Tensor& campos,
+                               int64_t degree, bool single) {
+    Guard guard(xyz.device());
+    if (wanted(xyz, features)) return ShColorsQuantizedFn::apply(xyz, features, campos, degree, single);
+    at::Tensor codes, scales, mask;
+    return quantized_of(xyz, features, campos, degree, single, codes, scales, mask);
+}
+
+at::Tensor keep_heaviest(const at::Tensor& weights, const std::vector<std::tuple<int, int, int, int>>& plan) {
+    Guard guard(weights.device());
+    std::vector<gsr_keep_group> g;
+    int64_t n = 0;
+    for (const auto& [a, b, k, r] : plan) {
+        g.push_back({a, b, k, r});
+        n += k;
+    }
+    at::Tensor ids = at::empty({n}, like(weights, at::kInt));
+    if (n) {
+        const int P = (int)weights.numel();
+        at::Tensor ws = at::empty({(int64_t)gsr_keep_ws_bytes(P)}, like(weights, at::kByte));
+        check(gsr_keep_heaviest(P, weights.data_ptr<float>(), (int)g.size(), g.data(), ids.data_ptr<int>(),
+                                ws.data_ptr(), cur_stream()));
+    }
+    return ids;
+}
+
+// compact.py _take: the tensors' checks, the outputs where none are given, one gsr_take_rows.
+std::vector<at::Tensor> take_rows(const at::Tensor& ids, const std::vector<at::Tensor>& tensors,
+                                  std::vector<at::Tensor> out, const std::vector<int>& pad, bool given) {
+    const int64_t K = ids.size(0);
+    auto fine = [&](const at::Tensor& t) {
+        return (t.scalar_type() == at::kFloat || t.scalar_type() == at::kInt) && t.dim() >= 1 && t.is_contiguous() &&
+               t.device() == ids.device() && t.size(0) < (1LL << 31);
+    };
+    auto refuse = [&](const char* name, size_t n) {
+        throw std::runtime_error("take_rows: " + std::string(name) + "[" + std::to_string(n) +
+                                 "] must be a contiguous float32 or int32 tensor of rows on " + ids.device().str());
+    };
+    Guard guard(ids.device());
+    std::vector<gsr_rows> table;
+    table.reserve(tensors.size());
+    for (size_t n = 0; n < tensors.size(); ++n) {
+        const at::Tensor& t = tensors[n];
+        if (!fine(t)) refuse("tensors", n);
+        int64_t width = 1;
+        for (int64_t d = 1; d < t.dim(); ++d) width *= t.size(d);
+        if (width > (1 << 20)) throw std::runtime_error("take_rows: rows of more than 2^20 values");
+        if (!given) {
+            std::vector<int64_t> shape = t.sizes().vec();
+            shape[0] = K;
+            out.push_back(at::empty(shape, t.options().requires_grad(false)));
+        } else {
+            const at::Tensor& o = out[n];
+            if (!fine(o)) refuse("out", n);
+            if (o.scalar_type() != t.scalar_type() || o.size(0) != K || o.sizes().slice(1) != t.sizes().slice(1))
+                throw std::runtime_error("take_rows: out[" + std::to_string(n) + "] must be " +
+                                         std::string(c10::toString(t.scalar_type())) + " of " + std::to_string(K) +
+                                         " rows like tensors[" + std::to_string(n) + "]");
+        }
+        table.push_back({t.data_ptr(), out[n].data_ptr(), (int)width, (int)t.size(0), pad.empty() ? 0 : pad[n]});
+    }
+    if (!table.empty()) check(gsr_take_rows((int)K, ids.data_ptr<int>(), (int)table.size(), table.data(), cur_stream()));
+    return out;
+}
+
+void bind_compact(pybind11::module_& mod) {
+    namespace py = pybind11;
+    mod.def("mx4_quantize", &mx4_quantize, py::call_guard<py::gil_scoped_release>());
+    mod.def("mx4_dequantize", &mx4_dequantize, py::call_guard<py::gil_scoped_release>());
+    mod.def("sh_colors", &sh_colors, py::call_guard<py::gil_scoped_release>());
+    mod.def("sh_colors_quantized", &sh_colors_quantized, py::call_guard<py::gil_scoped_release>());
+    mod.def("keep_heaviest", &keep_heaviest, py::call_guard<py::gil_scoped_release>());
+    mod.def("take_rows", &take_rows, py::call_guard<py::gil_scoped_release>());
+}

@@ -381,6 +381,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, int64_t> 
     return {o[0], o[1], o[2], o[3], o[4], nr};
 }
 
+void bind_compact(pybind11::module_& mod);  // host_compact.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {  // the single-view entry points of DGR/ext.cpp:15-19
     // the GIL is released for the whole call, as ctypes does for foreign calls: the forward
     // waits for num_rendered inside gsr_forward
@@ -401,4 +403,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {  // the single-view entry points of
     });
     mod.def("version", []() { return std::string(gsr_version()); });
     mod.def("lib_ns", []() { return (long long)g_lib_ns.load(); });
+    bind_compact(mod);
 }

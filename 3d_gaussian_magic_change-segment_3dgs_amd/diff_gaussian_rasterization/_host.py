@@ -1,5 +1,6 @@
 """The compiled host binding (csrc/host_ext.cpp, torch extension "gsr_host"): the single-view
-forward / backward host work of _C.py in C++ (argument checks, allocations, libgsr calls).
+forward / backward host work of _C.py in C++ (argument checks, allocations, libgsr calls), and that
+of the compact-scene operators (csrc/host_compact.cpp, used by gsr_train.compact).
 
 build() compiles it in-tree into build/ext_host/ (torch.utils.cpp_extension, host compiler, no
 hipify pass; linked against libgsr.so); __graft_entry__.build() runs it.  load() returns the
@@ -16,7 +17,8 @@ _PKG = os.path.dirname(_HERE)
 _ROOT = os.path.dirname(_PKG)
 BUILD = os.path.join(_ROOT, "build", "ext_host")
 NAME = "gsr_host"
-SOURCE = os.path.join(_PKG, "csrc", "host_ext.cpp")
+SOURCES = [os.path.join(_PKG, "csrc", f) for f in ("host_ext.cpp", "host_compact.cpp")]
+HEADERS = [os.path.join(_ROOT, "include", f) for f in ("gsr.h", "gsr_train.h", "gsr_compact.h")]
 
 
 def so_path():
@@ -26,7 +28,7 @@ def so_path():
 def source_digest():
     """Hash of the sources the module is built from (a stale build is not loaded)."""
     h = hashlib.sha256()
-    for p in (SOURCE, os.path.join(_ROOT, "include", "gsr.h"), os.path.join(_ROOT, "include", "gsr_train.h")):
+    for p in SOURCES + HEADERS:
         with open(p, "rb") as f:
             h.update(f.read())
     return h.hexdigest()[:16]
@@ -35,7 +37,7 @@ def source_digest():
 def build(verbose=False):
     import torch.utils.cpp_extension as ce
     os.makedirs(BUILD, exist_ok=True)
-    ce.load(name=NAME, sources=[SOURCE], build_directory=BUILD, with_cuda=False, verbose=verbose,
+    ce.load(name=NAME, sources=SOURCES, build_directory=BUILD, with_cuda=False, verbose=verbose,
             extra_include_paths=[os.path.join(_ROOT, "include"), "/opt/rocm/include"],
             extra_cflags=["-O2", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"],
             extra_ldflags=["-L" + _HERE, "-lgsr", "-Wl,-rpath," + _HERE, "-L/opt/rocm/lib", "-lamdhip64",

@@ -22,7 +22,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _C
-from diff_gaussian_rasterization._C import MAX_VIEWS
+from diff_gaussian_rasterization._C import MAX_VIEWS, _HOST
 
 _lib = _C._lib
 _vp, _i, _ll, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
@@ -116,6 +116,8 @@ class MX4Rows:
     def dequantize(self):
         """The values the codes stand for, float32 [rows, width] (each is exact)."""
         _on_gpu("MX4Rows.dequantize", self.codes)
+        if _HOST is not None:
+            return _HOST.mx4_dequantize(self.codes, self.scales, self.width)
         x = torch.empty((self.rows, self.width), dtype=torch.float32, device=self.device)
         if x.numel():
             _call(self.device, _lib.gsr_mx4_dequantize, self.rows, self.width, self.codes.data_ptr(),
@@ -128,6 +130,8 @@ class MX4Rows:
 
 def _quantize(x2):
     """x2 [R, K] with contiguous values in a row -> (codes, scales)."""
+    if _HOST is not None:
+        return _HOST.mx4_quantize(x2)
     R, K = x2.shape
     codes = torch.empty((R, 4 * _words(K)), dtype=torch.uint8, device=x2.device)
     scales = torch.empty((R, _blocks(K)), dtype=torch.uint8, device=x2.device)
@@ -147,14 +151,17 @@ def mx4_quantize(x):
     _on_gpu("mx4_quantize", x)
     if x.numel() and ((x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
         x = x.contiguous()
-    return MX4Rows(*_quantize(x), x.shape[1])
+    q = MX4Rows.__new__(MX4Rows)  # (nothing to check)
+    q.codes, q.scales = _quantize(x)
+    q.width = x.shape[1]
+    return q
 
 
 # ---- colours -----------------------------------------------------------------------------
 def _sh_check(what, xyz, campos, degree, M):
     _typed(what, xyz=xyz, campos=campos)
-    if xyz.dim() != 2 or xyz.shape[1] != 3:
-        raise RuntimeError(f"{what}: xyz must have shape (P, 3)")
+    if xyz.dim() != 2 or xyz.shape[1] != 3 or xyz.shape[0] >= 2 ** 31:
+        raise RuntimeError(f"{what}: xyz must have shape (P, 3), P below 2^31")
     if campos.shape != (3,) and (campos.dim() != 2 or campos.shape[1] != 3 or not 1 <= campos.shape[0] <= MAX_VIEWS):
         raise RuntimeError(f"{what}: campos must have shape (3,) or (V, 3) with V of 1..{MAX_VIEWS}")
     if int(degree) != degree or not 0 <= degree <= 3 or (degree + 1) ** 2 > M:
@@ -260,8 +267,9 @@ def sh_colors(xyz, features_dc, rest, campos, degree):
     dc = features_dc.reshape(P, 3)
     if P and (dc.stride(1) != 1 or (P > 1 and dc.stride(0) < 3)):
         dc = dc.contiguous()
-    return _ShColors.apply(xyz.contiguous(), dc, campos.detach().reshape(-1, 3).contiguous(), rest.codes, rest.scales,
-                           int(degree), M, campos.dim() == 1)
+    fn = _ShColors.apply if _HOST is None else _HOST.sh_colors
+    return fn(xyz.contiguous(), dc, campos.detach().reshape(-1, 3).contiguous(), rest.codes, rest.scales, int(degree), M,
+              campos.dim() == 1)
 
 
 def sh_colors_quantized(xyz, features, campos, degree):
@@ -277,8 +285,9 @@ def sh_colors_quantized(xyz, features, campos, degree):
     if features.shape[0] != xyz.shape[0]:
         raise RuntimeError(f"{what}: features must have {xyz.shape[0]} rows (got {features.shape[0]})")
     _on_gpu(what, xyz, features=features, campos=campos)
-    return _ShColorsQuantized.apply(xyz.contiguous(), features.contiguous(),
-                                    campos.detach().reshape(-1, 3).contiguous(), int(degree), campos.dim() == 1)
+    fn = _ShColorsQuantized.apply if _HOST is None else _HOST.sh_colors_quantized
+    return fn(xyz.contiguous(), features.contiguous(), campos.detach().reshape(-1, 3).contiguous(), int(degree),
+              campos.dim() == 1)
 
 
 # ---- eviction to a budget --------------------------------------------------------------------
@@ -329,9 +338,13 @@ def keep_heaviest(weights, budgets, groups=None, recent=0):
     equals the lowest row; NaN counts as lighter than everything.  Rows in no group go."""
     _typed("keep_heaviest", weights=weights)
     P = weights.numel()
+    if P >= 2 ** 31:
+        raise RuntimeError("keep_heaviest: at most 2^31 - 1 weights")
     plan = _keep_groups("keep_heaviest", P, budgets, groups, recent)
     _on_gpu("keep_heaviest", weights)
     weights = weights.contiguous()
+    if _HOST is not None:
+        return _HOST.keep_heaviest(weights, plan)
     ids = torch.empty(sum(k for _, _, k, _ in plan), dtype=torch.int32, device=weights.device)
     if ids.numel():
         ws = torch.empty(int(_lib.gsr_keep_ws_bytes(P)), dtype=torch.uint8, device=weights.device)
@@ -349,20 +362,25 @@ def take_rows(ids, tensors, out=None):
     _typed("take_rows", torch.int32, ids=ids)
     if ids.dim() != 1 or not ids.is_contiguous():
         raise RuntimeError("take_rows: ids must be contiguous, of shape (K,)")
-    tensors = list(tensors)
-    return _take(ids, tensors, [torch.empty((ids.shape[0],) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device)
-                                for t in tensors] if out is None else list(out), [0] * len(tensors))
+    return _take(ids, list(tensors), None if out is None else list(out), None)
 
 
 def _take(ids, tensors, out, pad):
     K = ids.shape[0]
-    if len(out) != len(tensors):
+    if out is not None and len(out) != len(tensors):
         raise RuntimeError("take_rows: one output for each tensor")
+    if _HOST is not None and ids.device.type == "cuda" and \
+            all(isinstance(t, torch.Tensor) for t in tensors + (out or [])):
+        got = _HOST.take_rows(ids, tensors, out or [], pad or [], out is not None)
+        return got if out is None else out
+    if out is None:
+        out = [torch.empty((K,) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device) if isinstance(t, torch.Tensor)
+               else None for t in tensors]
     table = (_Rows * len(tensors))()
     for n, (t, o) in enumerate(zip(tensors, out)):
         for x, name in ((t, "tensors"), (o, "out")):
             if not isinstance(x, torch.Tensor) or x.dtype not in (torch.float32, torch.int32) or x.dim() < 1 or \
-                    not x.is_contiguous() or x.device != ids.device:
+                    not x.is_contiguous() or x.device != ids.device or x.shape[0] >= 2 ** 31:
                 raise RuntimeError(f"take_rows: {name}[{n}] must be a contiguous float32 or int32 tensor of rows on "
                                    f"{ids.device}")
         if o.dtype != t.dtype or o.shape[0] != K or o.shape[1:] != t.shape[1:]:
@@ -370,7 +388,9 @@ def _take(ids, tensors, out, pad):
         width = 1
         for d in t.shape[1:]:
             width *= d
-        table[n] = (t.data_ptr(), o.data_ptr(), width, t.shape[0], pad[n])
+        if width > 1 << 20:
+            raise RuntimeError("take_rows: rows of more than 2^20 values")
+        table[n] = (t.data_ptr(), o.data_ptr(), width, t.shape[0], pad[n] if pad else 0)
     _on_gpu("take_rows", ids)
     if tensors:
         _call(ids.device, _lib.gsr_take_rows, K, ids.data_ptr(), len(tensors), table)

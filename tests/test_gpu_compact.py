@@ -275,7 +275,50 @@ def test_colors_empty_and_not_contiguous():
     assert torch.equal(gs, ho)
 
 
-def test_colors_double_backward_is_refused():
+def both_routes(monkeypatch):
+    """The C++ host binding and ctypes in turn."""
+    from gsr_train import compact as T
+    assert T._HOST is not None, "gsr_host not built (__graft_entry__.build())"
+    yield "host"
+    monkeypatch.setattr(T, "_HOST", None)
+    yield "ctypes"
+
+
+def test_both_host_routes_give_the_same(monkeypatch):
+    import gsr_train as G
+    xyz, f, cam, up = scene(3000, 16, 3, 12)
+    w = torch.exp(torch.randn(50_000, generator=gen(1))).to(DEV)
+    rows = [torch.randn(50_000, k, generator=gen(k)).to(DEV) for k in (1, 3, 48)]
+    got = {}
+    for route in both_routes(monkeypatch):
+        x, fg = xyz.to(DEV).requires_grad_(), f.to(DEV).requires_grad_()
+        q = G.mx4_quantize(fg.detach().flatten(1)[:, 3:])
+        dc = f[:, 0].to(DEV).requires_grad_()
+        a = G.sh_colors_quantized(x, fg, cam.to(DEV), 3)
+        b = G.sh_colors(x, dc, q, cam.to(DEV), 3)
+        assert a.requires_grad and b.requires_grad
+        with torch.no_grad():
+            c = G.sh_colors_quantized(x, fg, cam.to(DEV), 3)
+        assert not c.requires_grad and not G.sh_colors(x.detach(), dc.detach(), q, cam.to(DEV), 3).requires_grad
+        ids = G.keep_heaviest(w, [100, 20_000], [(0, 5000), (5000, 50_000)], 7)
+        got[route] = [q.codes, q.scales, q.dequantize(), a, b, c, ids, *G.take_rows(ids, rows),
+                      *torch.autograd.grad(a, (x, fg), up.to(DEV)), *torch.autograd.grad(b, (x, dc), up.to(DEV))]
+        with pytest.raises(RuntimeError, match="tensors.1. must be"):
+            G.take_rows(ids, [rows[0], rows[1].double()])
+        with pytest.raises(RuntimeError, match="out.0. must be"):
+            G.take_rows(ids, [rows[0]], out=[rows[1]])
+        with pytest.raises(RuntimeError, match="contiguous"):
+            G.take_rows(ids, [rows[2][:, ::2]])
+    for a, b in zip(got["host"], got["ctypes"]):
+        assert a.shape == b.shape and torch.equal(a, b)
+
+
+def test_colors_double_backward_is_refused(monkeypatch):
+    for _ in both_routes(monkeypatch):
+        check_double_backward()
+
+
+def check_double_backward():
     import gsr_train as G
     xyz, f, cam, up = scene(10, 4, 1, 3)
     x = xyz.to(DEV).requires_grad_()
