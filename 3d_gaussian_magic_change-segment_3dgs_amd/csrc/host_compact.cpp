@@ -1,8 +1,7 @@
 // host_compact.cpp -- the host side of the compact-scene operators in C++ (part of the torch
 // extension "gsr_host"): allocation, the libgsr calls of include/gsr_compact.h and the autograd
-// functions, as gsr_train/compact.py does them over ctypes.  The Python layer checks the arguments of
-// the single operators before it calls in here (take_rows, whose tensors are many, is checked here);
-// a training step of colours costs ~90 us of host time less than through Python's autograd.
+// functions, as gsr_train/compact.py does them over ctypes, with its checks and messages: small calls
+// are bound by the host (10k Gaussians: colours 18 us through Python and ctypes, 3 us on the GPU).
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
@@ -34,8 +33,33 @@ uint32_t* code_out(at::Tensor& t) { return reinterpret_cast<uint32_t*>(t.data_pt
 
 }  // namespace
 
-std::tuple<at::Tensor, at::Tensor> mx4_quantize(const at::Tensor& x) {
-    Guard guard(x.device());
+namespace {
+
+[[noreturn]] void refuse(const std::string& text) { throw std::runtime_error(text); }
+
+void check_float(const char* what, const char* name, const at::Tensor& t) {
+    if (t.scalar_type() != at::kFloat)
+        refuse(std::string(what) + ": " + name + " must be a torch.float32 tensor (got " +
+               c10::toString(t.scalar_type()) + ")");
+}
+void check_gpu(const char* what, const at::Tensor& t) {
+    if (!t.is_cuda()) refuse(std::string(what) + ": tensors must be on the GPU (the HIP path has no CPU fallback)");
+}
+void check_device(const char* what, const char* name, const at::Tensor& t, const at::Tensor& first) {
+    if (t.device() != first.device())
+        refuse(std::string(what) + ": " + name + " is on " + t.device().str() + ", expected " + first.device().str());
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> mx4_quantize(const at::Tensor& rows) {
+    check_float("mx4_quantize", "x", rows);
+    if (rows.dim() != 2) refuse("mx4_quantize: x must have shape (rows, values)");
+    check_gpu("mx4_quantize", rows);
+    Guard guard(rows.device());
+    const bool apart = rows.numel() && ((rows.size(1) > 1 && rows.stride(1) != 1) ||
+                                        (rows.size(0) > 1 && rows.stride(0) < rows.size(1)));
+    const at::Tensor x = apart ? rows.contiguous() : rows;
     const int64_t R = x.size(0), K = x.size(1);
     at::Tensor codes = at::empty({R, 4 * words(K)}, like(x, at::kByte));
     at::Tensor scales = at::empty({R, blocks(K)}, like(x, at::kByte));
@@ -168,16 +192,68 @@ bool wanted(const at::Tensor& a, const at::Tensor& b) {
 
 }  // namespace
 
-at::Tensor sh_colors(const at::Tensor& xyz, const at::Tensor& dc, const at::Tensor& campos, const at::Tensor& codes,
-                     const at::Tensor& scales, int64_t degree, int64_t M, bool single) {
-    Guard guard(xyz.device());
+namespace {
+void check_sh(const char* what, const at::Tensor& xyz, const at::Tensor& campos, int64_t degree, int64_t M) {
+    check_float(what, "xyz", xyz);
+    check_float(what, "campos", campos);
+    if (xyz.dim() != 2 || xyz.size(1) != 3 || xyz.size(0) >= (1LL << 31))
+        refuse(std::string(what) + ": xyz must have shape (P, 3), P below 2^31");
+    const bool one = campos.dim() == 1 && campos.size(0) == 3;
+    const bool many = campos.dim() == 2 && campos.size(1) == 3 && campos.size(0) >= 1 && campos.size(0) <= GSR_MAX_VIEWS;
+    if (!one && !many)
+        refuse(std::string(what) + ": campos must have shape (3,) or (V, 3) with V of 1.." + std::to_string(GSR_MAX_VIEWS));
+    if (degree < 0 || degree > 3 || (degree + 1) * (degree + 1) > M)
+        refuse(std::string(what) + ": degree must be 0..3 and the features must hold its coefficients (degree " +
+               std::to_string(degree) + ", " + std::to_string(M) + " coefficients)");
+}
+at::Tensor views_of(const at::Tensor& campos) {
+    const at::Tensor c = campos.requires_grad() ? campos.detach() : campos;
+    return (c.dim() == 1 ? c.unsqueeze(0) : c).contiguous();
+}
+}  // namespace
+
+at::Tensor sh_colors(const at::Tensor& xyz_, const at::Tensor& features_dc, const at::Tensor& codes,
+                     const at::Tensor& scales, int64_t width, const at::Tensor& campos_, int64_t degree) {
+    if (width % 3 || width > 45) refuse("sh_colors: rest must be MX4Rows of 3 (M - 1) values, M of 1..16");
+    const int64_t M = width / 3 + 1;
+    check_sh("sh_colors", xyz_, campos_, degree, M);
+    check_float("sh_colors", "features_dc", features_dc);
+    const int64_t P = xyz_.size(0), dims = features_dc.dim();
+    if (!((dims == 2 || (dims == 3 && features_dc.size(1) == 1)) && features_dc.size(0) == P &&
+          features_dc.size(dims - 1) == 3))
+        refuse("sh_colors: features_dc must have shape (" + std::to_string(P) + ", 1, 3) or (" + std::to_string(P) +
+               ", 3)");
+    if (codes.size(0) != P)
+        refuse("sh_colors: rest must have " + std::to_string(P) + " rows (got " + std::to_string(codes.size(0)) + ")");
+    check_gpu("sh_colors", xyz_);
+    check_device("sh_colors", "features_dc", features_dc, xyz_);
+    check_device("sh_colors", "rest", codes, xyz_);
+    check_device("sh_colors", "campos", campos_, xyz_);
+    Guard guard(xyz_.device());
+    const bool single = campos_.dim() == 1;
+    const at::Tensor xyz = xyz_.contiguous(), campos = views_of(campos_);
+    at::Tensor dc = dims == 3 ? features_dc.squeeze(1) : features_dc;
+    if (P && (dc.stride(1) != 1 || (P > 1 && dc.stride(0) < 3))) dc = dc.contiguous();
     if (wanted(xyz, dc)) return ShColorsFn::apply(xyz, dc, campos, codes, scales, degree, M, single);
     return colors_of(xyz, dc, campos, codes, scales, degree, M, single, nullptr);
 }
 
-at::Tensor sh_colors_quantized(const at::Tensor& xyz, const at::Tensor& features, const at::Tensor& campos,
-                               int64_t degree, bool single) {
-    Guard guard(xyz.device());
+at::Tensor sh_colors_quantized(const at::Tensor& xyz_, const at::Tensor& features_, const at::Tensor& campos_,
+                               int64_t degree) {
+    const char* what = "sh_colors_quantized";
+    check_float(what, "features", features_);
+    if (features_.dim() != 3 || features_.size(2) != 3 || features_.size(1) < 1 || features_.size(1) > 16)
+        refuse(std::string(what) + ": features must have shape (P, M, 3), M of 1..16");
+    check_sh(what, xyz_, campos_, degree, features_.size(1));
+    if (features_.size(0) != xyz_.size(0))
+        refuse(std::string(what) + ": features must have " + std::to_string(xyz_.size(0)) + " rows (got " +
+               std::to_string(features_.size(0)) + ")");
+    check_gpu(what, xyz_);
+    check_device(what, "features", features_, xyz_);
+    check_device(what, "campos", campos_, xyz_);
+    Guard guard(xyz_.device());
+    const bool single = campos_.dim() == 1;
+    const at::Tensor xyz = xyz_.contiguous(), features = features_.contiguous(), campos = views_of(campos_);
     if (wanted(xyz, features)) return ShColorsQuantizedFn::apply(xyz, features, campos, degree, single);
     at::Tensor codes, scales, mask;
     return quantized_of(xyz, features, campos, degree, single, codes, scales, mask);
@@ -209,30 +285,29 @@ std::vector<at::Tensor> take_rows(const at::Tensor& ids, const std::vector<at::T
         return (t.scalar_type() == at::kFloat || t.scalar_type() == at::kInt) && t.dim() >= 1 && t.is_contiguous() &&
                t.device() == ids.device() && t.size(0) < (1LL << 31);
     };
-    auto refuse = [&](const char* name, size_t n) {
-        throw std::runtime_error("take_rows: " + std::string(name) + "[" + std::to_string(n) +
-                                 "] must be a contiguous float32 or int32 tensor of rows on " + ids.device().str());
+    auto bad = [&](const char* name, size_t n) {
+        refuse("take_rows: " + std::string(name) + "[" + std::to_string(n) +
+               "] must be a contiguous float32 or int32 tensor of rows on " + ids.device().str());
     };
     Guard guard(ids.device());
     std::vector<gsr_rows> table;
     table.reserve(tensors.size());
     for (size_t n = 0; n < tensors.size(); ++n) {
         const at::Tensor& t = tensors[n];
-        if (!fine(t)) refuse("tensors", n);
+        if (!fine(t)) bad("tensors", n);
         int64_t width = 1;
         for (int64_t d = 1; d < t.dim(); ++d) width *= t.size(d);
-        if (width > (1 << 20)) throw std::runtime_error("take_rows: rows of more than 2^20 values");
+        if (width > (1 << 20)) refuse("take_rows: rows of more than 2^20 values");
         if (!given) {
             std::vector<int64_t> shape = t.sizes().vec();
             shape[0] = K;
             out.push_back(at::empty(shape, t.options().requires_grad(false)));
         } else {
             const at::Tensor& o = out[n];
-            if (!fine(o)) refuse("out", n);
+            if (!fine(o)) bad("out", n);
             if (o.scalar_type() != t.scalar_type() || o.size(0) != K || o.sizes().slice(1) != t.sizes().slice(1))
-                throw std::runtime_error("take_rows: out[" + std::to_string(n) + "] must be " +
-                                         std::string(c10::toString(t.scalar_type())) + " of " + std::to_string(K) +
-                                         " rows like tensors[" + std::to_string(n) + "]");
+                refuse("take_rows: out[" + std::to_string(n) + "] must be " + c10::toString(t.scalar_type()) + " of " +
+                       std::to_string(K) + " rows like tensors[" + std::to_string(n) + "]");
         }
         table.push_back({t.data_ptr(), out[n].data_ptr(), (int)width, (int)t.size(0), pad.empty() ? 0 : pad[n]});
     }

@@ -130,8 +130,6 @@ class MX4Rows:
 
 def _quantize(x2):
     """x2 [R, K] with contiguous values in a row -> (codes, scales)."""
-    if _HOST is not None:
-        return _HOST.mx4_quantize(x2)
     R, K = x2.shape
     codes = torch.empty((R, 4 * _words(K)), dtype=torch.uint8, device=x2.device)
     scales = torch.empty((R, _blocks(K)), dtype=torch.uint8, device=x2.device)
@@ -140,19 +138,22 @@ def _quantize(x2):
     return codes, scales
 
 
-@torch.no_grad()
 def mx4_quantize(x):
     """Rows of a float32 GPU tensor [R, K] -> MX4Rows (blocks of 32 neighbours of a row;
     the conversion is described in include/gsr_compact.h).  A view whose rows lie apart
     (features[:, 1:].flatten(1)) is read in place."""
-    _typed("mx4_quantize", x=x)
-    if x.dim() != 2:
-        raise RuntimeError("mx4_quantize: x must have shape (rows, values)")
-    _on_gpu("mx4_quantize", x)
-    if x.numel() and ((x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
-        x = x.contiguous()
+    if _HOST is not None and isinstance(x, torch.Tensor):
+        codes, scales = _HOST.mx4_quantize(x)
+    else:
+        _typed("mx4_quantize", x=x)
+        if x.dim() != 2:
+            raise RuntimeError("mx4_quantize: x must have shape (rows, values)")
+        _on_gpu("mx4_quantize", x)
+        if x.numel() and ((x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
+            x = x.contiguous()
+        codes, scales = _quantize(x)
     q = MX4Rows.__new__(MX4Rows)  # (nothing to check)
-    q.codes, q.scales = _quantize(x)
+    q.codes, q.scales = codes, scales
     q.width = x.shape[1]
     return q
 
@@ -244,6 +245,12 @@ class _ShColorsQuantized(torch.autograd.Function):
         return dxyz, df, None, None, None
 
 
+def _plain(a, b, c, degree):
+    """What the C++ binding takes; anything else is refused (or converted) below."""
+    return isinstance(a, torch.Tensor) and isinstance(b, torch.Tensor) and isinstance(c, torch.Tensor) and \
+        type(degree) is int
+
+
 def sh_colors(xyz, features_dc, rest, campos, degree):
     """max(0, 1/2 + sum_k Y_k(d) coefficient_k), d the direction from the camera to the
     Gaussian, for coefficients held in 4 bits (utils/sh_utils.py:57-112 and the + 0.5 and
@@ -253,6 +260,8 @@ def sh_colors(xyz, features_dc, rest, campos, degree):
     values, campos [3] -> colors [P, 3], or [V, 3] -> [V, P, 3].  Differentiable in xyz and
     features_dc (gradients summed over the views); a channel that the clamp holds at zero
     gives no gradient, and a Gaussian at the camera position itself none to xyz."""
+    if _HOST is not None and isinstance(rest, MX4Rows) and _plain(xyz, features_dc, campos, degree):
+        return _HOST.sh_colors(xyz, features_dc, rest.codes, rest.scales, rest.width, campos, degree)
     if not isinstance(rest, MX4Rows) or rest.width % 3 or rest.width > 45:
         raise RuntimeError("sh_colors: rest must be MX4Rows of 3 (M - 1) values, M of 1..16")
     M = rest.width // 3 + 1
@@ -267,9 +276,8 @@ def sh_colors(xyz, features_dc, rest, campos, degree):
     dc = features_dc.reshape(P, 3)
     if P and (dc.stride(1) != 1 or (P > 1 and dc.stride(0) < 3)):
         dc = dc.contiguous()
-    fn = _ShColors.apply if _HOST is None else _HOST.sh_colors
-    return fn(xyz.contiguous(), dc, campos.detach().reshape(-1, 3).contiguous(), rest.codes, rest.scales, int(degree), M,
-              campos.dim() == 1)
+    return _ShColors.apply(xyz.contiguous(), dc, campos.detach().reshape(-1, 3).contiguous(), rest.codes, rest.scales,
+                           int(degree), M, campos.dim() == 1)
 
 
 def sh_colors_quantized(xyz, features, campos, degree):
@@ -277,6 +285,8 @@ def sh_colors_quantized(xyz, features, campos, degree):
     coefficients above the constant one are rounded to 4 bits in the call: the colours a
     model shows after `compact()`.  Differentiable in xyz and features; the gradient goes
     straight through the rounding, and coefficients above `degree` get zero."""
+    if _HOST is not None and _plain(xyz, features, campos, degree):
+        return _HOST.sh_colors_quantized(xyz, features, campos, degree)
     what = "sh_colors_quantized"
     _typed(what, features=features)
     if features.dim() != 3 or features.shape[2] != 3 or not 1 <= features.shape[1] <= 16:
@@ -285,9 +295,8 @@ def sh_colors_quantized(xyz, features, campos, degree):
     if features.shape[0] != xyz.shape[0]:
         raise RuntimeError(f"{what}: features must have {xyz.shape[0]} rows (got {features.shape[0]})")
     _on_gpu(what, xyz, features=features, campos=campos)
-    fn = _ShColorsQuantized.apply if _HOST is None else _HOST.sh_colors_quantized
-    return fn(xyz.contiguous(), features.contiguous(), campos.detach().reshape(-1, 3).contiguous(), int(degree),
-              campos.dim() == 1)
+    return _ShColorsQuantized.apply(xyz.contiguous(), features.contiguous(),
+                                    campos.detach().reshape(-1, 3).contiguous(), int(degree), campos.dim() == 1)
 
 
 # ---- eviction to a budget --------------------------------------------------------------------
@@ -327,7 +336,6 @@ def _keep_groups(what, P, budgets, groups, recent):
     return out
 
 
-@torch.no_grad()
 def keep_heaviest(weights, budgets, groups=None, recent=0):
     """The rows that stay when each group is brought to its budget, int32, ascending.
 
@@ -353,7 +361,6 @@ def keep_heaviest(weights, budgets, groups=None, recent=0):
     return ids
 
 
-@torch.no_grad()
 def take_rows(ids, tensors, out=None):
     """[t[ids] for t in tensors] in one launch: ids int32 [K], tensors contiguous float32 or
     int32 of any shape [rows, ...] on the same GPU; `out`, if given, contiguous tensors of

@@ -63,8 +63,15 @@ def refused(fn, *a, match, **k):
         fn(*a, **k)
 
 
-def test_python_refusals():
+@pytest.mark.parametrize("route", ["host", "ctypes"])
+def test_python_refusals(route, monkeypatch):
+    """Both host routes, each with its own checks and the same messages."""
     import gsr_train as G
+    from gsr_train import compact as T
+    if route == "host" and T._HOST is None:
+        pytest.skip("gsr_host not built from these sources (__graft_entry__.build())")
+    if route == "ctypes":
+        monkeypatch.setattr(T, "_HOST", None)
     z = torch.zeros
     refused(G.mx4_quantize, z(4, 45), match="GPU")
     refused(G.mx4_quantize, z(4, 45, dtype=torch.float16), match="float32")
