@@ -602,6 +602,7 @@ struct KeepArgs {
 };
 struct KeepSel {
     uint32_t prefix, need;  // digits found so far; the rank looked for among the keys that share them
+    uint32_t count;         // how many those are
 };
 struct KeepWs {
     uint32_t* hist;  // [groups][3][KEEP_BINS]
@@ -672,23 +673,15 @@ __device__ __forceinline__ KeepSel find_bin(const uint32_t* hist, uint32_t need,
     uint32_t above = block_scan_excl<THREADS>(sum, s_wave);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-        if (above < need && need <= above + h[k]) *s_out = {(uint32_t)(top - k), need - above};
+        if (above < need && need <= above + h[k]) *s_out = {(uint32_t)(top - k), need - above, h[k]};
         above += h[k];
     }
     __syncthreads();
     return *s_out;
 }
 
-// Counts digit d of the active lanes; lanes that share one digit (equal weights) add as one.
 __device__ __forceinline__ void keep_add(uint32_t* h, uint32_t d, bool in) {
-    const unsigned long long act = __ballot(in);
-    if (act == 0) return;
-    const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)d, __builtin_ctzll(act));
-    if (__ballot(in && d == d0) == act) {
-        if ((threadIdx.x & 63) == 0) atomicAdd(&h[d0], (uint32_t)__popcll(act));
-    } else if (in) {
-        atomicAdd(&h[d], 1u);
-    }
+    if (in) atomicAdd(&h[d], 1u);
 }
 
 // Keys [i, i + 16) of rows below `end` (0 behind it).
@@ -733,7 +726,7 @@ __device__ __forceinline__ KeepSel keep_small_pass(const uint32_t (&key)[16], in
     }
     __syncthreads();
     const KeepSel b = find_bin<KEEP_SMALL_THREADS>(h, st.need, s_wave, s_out);
-    return {(st.prefix << (PASS == 2 ? 10 : 11)) | b.prefix, b.need};
+    return {(st.prefix << (PASS == 2 ? 10 : 11)) | b.prefix, b.need, b.count};
 }
 
 __global__ void __launch_bounds__(KEEP_SMALL_THREADS) k_keep_small(KeepArgs a, const float* __restrict__ w,
@@ -746,10 +739,15 @@ __global__ void __launch_bounds__(KEEP_SMALL_THREADS) k_keep_small(KeepArgs a, c
     if (G.pick > 0) {  // the whole block
         uint32_t key[16];
         keep_load16(w, (long long)G.begin + first, G.old_end, key);
-        KeepSel st = {0u, (uint32_t)G.pick};
+        KeepSel st = {0u, (uint32_t)G.pick, 0u};
         st = keep_small_pass<0>(key, n, st, h, s_wave, &s_out);
         st = keep_small_pass<1>(key, n, st, h, s_wave, &s_out);
-        st = keep_small_pass<2>(key, n, st, h, s_wave, &s_out);
+        if (st.count == st.need && st.prefix > 0) {  // all that share 22 bits stay: T just below them, no ties
+            st.prefix = (st.prefix << 10) - 1;
+            st.need = 0;
+        } else {
+            st = keep_small_pass<2>(key, n, st, h, s_wave, &s_out);
+        }
         uint32_t gt = 0, eq = 0;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -781,11 +779,11 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_clear(uint32_t* __restrict_
 template <int PASS>
 __device__ __forceinline__ KeepSel keep_state(const KeepArgs& a, const KeepWs& ws, int g, int tile, uint32_t* s_wave,
                                               KeepSel* s_out) {
-    KeepSel prev = {0u, (uint32_t)a.g[g].pick};
+    KeepSel prev = {0u, (uint32_t)a.g[g].pick, 0u};
     if constexpr (PASS == 0) return prev;
     if (PASS > 1) prev = ws.sel[g * 3 + PASS - 2];
     const KeepSel b = find_bin<CP_THREADS>(ws.hist + ((size_t)g * 3 + PASS - 1) * KEEP_BINS, prev.need, s_wave, s_out);
-    const KeepSel now = {(prev.prefix << (PASS == 3 ? 10 : 11)) | b.prefix, b.need};
+    const KeepSel now = {(prev.prefix << (PASS == 3 ? 10 : 11)) | b.prefix, b.need, b.count};
     if (tile == a.g[g].tile0 && threadIdx.x == 0) ws.sel[g * 3 + PASS - 1] = now;
     return now;
 }
@@ -844,7 +842,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_count(KeepArgs a, KeepWs ws
 __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws, const float* __restrict__ w,
                                                            int* __restrict__ ids) {
     __shared__ uint32_t s_wave[CP_THREADS / 64];
-    __shared__ unsigned long long s_sum;
+    __shared__ uint32_t s_gt, s_eq;
     __shared__ int s_ids[KEEP_TILE];
     __shared__ uint32_t s_n;
     const int tile = blockIdx.x, g = keep_group_of(a, tile);
@@ -854,20 +852,26 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
         uint32_t key[16];
         keep_load16(w, first, G.old_end, key);
         const KeepSel st = ws.sel[g * 3 + 2];
-        if (threadIdx.x == 0) s_sum = 0;
+        if (threadIdx.x == 0) s_gt = s_eq = 0;
         __syncthreads();
-        unsigned long long sum = 0;
+        uint2 sum = {0u, 0u};
         for (int t = G.tile0 + threadIdx.x; t < tile; t += CP_THREADS) {
             const uint2 c = ws.count[t];
-            sum += c.x | (unsigned long long)c.y << 32;
+            sum.x += c.x;
+            sum.y += c.y;
         }
-        if (sum) atomicAdd(&s_sum, sum);
+        sum.x = wave_scan(sum.x);
+        sum.y = wave_scan(sum.y);
+        if ((threadIdx.x & 63) == 63) {
+            atomicAdd(&s_gt, sum.x);
+            atomicAdd(&s_eq, sum.y);
+        }
         uint32_t both = 0;
 #pragma unroll
         for (int k = 0; k < 16; ++k)
             if (first + k < G.old_end) both += key[k] > st.prefix ? 1u : key[k] == st.prefix ? 1u << 16 : 0u;
         const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave);  // (its barriers also end the sum)
-        const uint32_t gt0 = (uint32_t)s_sum, eq0 = (uint32_t)(s_sum >> 32);
+        const uint32_t gt0 = s_gt, eq0 = s_eq;
         const uint32_t ties = eq0 < st.need ? st.need - eq0 : 0u;  // left for this tile
         uint32_t gt = before & 0xFFFFu, eq = before >> 16;
 #pragma unroll
