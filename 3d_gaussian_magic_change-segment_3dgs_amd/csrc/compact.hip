@@ -388,13 +388,24 @@ constexpr int ROW16 = 13;                  // float4s
 constexpr int ROWS_LDS = 64 * 4 * ROW16;   // floats a wave (also 64 rows of 45)
 __device__ __forceinline__ void wave_lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// With NT the rows pass by the caches: what those hold of a tensor that does not fit them is gone
+// before its next reader comes, and was in the way of other data until then.  Loads of 192 MB of
+// features (1M Gaussians, one view): forward 50 -> 43 us; of 58 MB (300k): 14.0 -> 15.2, so not there.
+// Stores of the gradient: 192 MB, backward 49 -> 39 us; 58 MB and 8 views, 31 -> 24.
+constexpr long long NT_LOAD_BYTES = 128LL << 20, NT_STORE_BYTES = 32LL << 20;
+template <bool NT>
 __device__ __forceinline__ void rows_in(const float* __restrict__ src, int rows, int F, float* lds, int lane) {
     if (F == 48) {
         v4a v[12];
 #pragma unroll
         for (int r = 0; r < 12; ++r) {
             const int f = lane + 64 * r;
-            v[r] = f / 12 < rows ? *reinterpret_cast<const v4a*>(src + 4 * f) : v4a{0.0f, 0.0f, 0.0f, 0.0f};
+            const v4a* q = reinterpret_cast<const v4a*>(src + 4 * f);
+            v[r] = v4a{0.0f, 0.0f, 0.0f, 0.0f};
+            if (f / 12 < rows) {
+                if constexpr (NT) v[r] = __builtin_nontemporal_load(q);
+                else v[r] = *q;
+            }
         }
         float4* d = reinterpret_cast<float4*>(lds);
 #pragma unroll
@@ -412,6 +423,7 @@ __device__ __forceinline__ void rows_in(const float* __restrict__ src, int rows,
     wave_lds_wait();
 }
 
+template <bool NT>
 __device__ __forceinline__ void rows_out(float* __restrict__ dst, int rows, int F, const float* lds, int lane) {
     wave_lds_wait();
     if (F == 48) {
@@ -420,7 +432,12 @@ __device__ __forceinline__ void rows_out(float* __restrict__ dst, int rows, int 
         for (int r = 0; r < 12; ++r) {
             const int f = lane + 64 * r;
             const float4 v = d[f / 12 * ROW16 + f % 12];
-            if (f / 12 < rows) *reinterpret_cast<v4a*>(dst + 4 * f) = v4a{v.x, v.y, v.z, v.w};
+            v4a* q = reinterpret_cast<v4a*>(dst + 4 * f);
+            const v4a o = {v.x, v.y, v.z, v.w};
+            if (f / 12 < rows) {
+                if constexpr (NT) __builtin_nontemporal_store(o, q);
+                else *q = o;
+            }
         }
     } else {
         const int n = (rows < 64 ? rows : 64) * F;
@@ -440,7 +457,7 @@ __device__ __forceinline__ void rows_out(float* __restrict__ dst, int rows, int 
 // Training forward: a Gaussian's fp32 coefficients are read once, rounded to codes (kept for the
 // backward), read back and evaluated.  The blocks that the degree touches are rounded whole, so a
 // code does not depend on the degree.
-template <int DEG>
+template <int DEG, bool NT>
 __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, const float* __restrict__ features,
                                                                    uint32_t* __restrict__ codes,
                                                                    uint8_t* __restrict__ scales,
@@ -452,7 +469,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, con
     const int first = blockIdx.x * CP_THREADS + wave * 64, i = first + lane, F = 3 * a.M;
     if (first >= a.P) return;  // the whole wave
     float* lds = reinterpret_cast<float*>(s_rows[wave]);
-    rows_in(features + (long long)first * F, a.P - first, F, lds, lane);
+    rows_in<NT>(features + (long long)first * F, a.P - first, F, lds, lane);
     if (i >= a.P) return;
     constexpr int VALUES = C::BLOCKS * GSR_MX_BLOCK;  // of the row behind its constant coefficient
     float v[VALUES + 3];
@@ -506,7 +523,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, con
 // channels take part comes from the forward's mask, so the constant coefficients (whose basis value
 // has no slope) are not read.
 // WANT_F: dfeatures is wanted (else at most its first coefficient, ddc).
-template <int DEG, bool WANT_F>
+template <int DEG, bool WANT_F, bool NT>
 __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, const uint8_t* __restrict__ mask,
                                                                    const float* __restrict__ dcolors,
                                                                    float* __restrict__ dxyz, float* __restrict__ ddc,
@@ -566,7 +583,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, con
             for (int k = 0; k < 3 * N; ++k) lds[lane * F + k] = acc[k];
             for (int k = 3 * N; k < F; ++k) lds[lane * F + k] = 0.0f;
         }
-        rows_out(dfeatures + (long long)first * F, a.P - first, F, lds, lane);
+        rows_out<NT>(dfeatures + (long long)first * F, a.P - first, F, lds, lane);
     }
 }
 
@@ -895,7 +912,9 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
 // ------------------------------------------------------------------------ rows --
 // A copy: K rows of each tensor read and written once, bound by memory.  A block moves
 // TAKE_SPAN units of one tensor's output, a unit being 16 bytes where the rows are whole
-// float4s (the features, 48 of a Gaussian's 61 floats, and the rotations), else 4.
+// float4s (the features, 48 of a Gaussian's 61 floats, and the rotations), else 4.  Loads and
+// wide stores pass by the caches: every line is wanted by one instruction (1M rows of 732 bytes
+// kept at 70 %: 215 us with temporal ones, 198 so, 5.2 TB/s).
 constexpr int TAKE_MAX = 32;    // tensors a launch
 constexpr int TAKE_PER = 4;     // units a thread: their ids, then their values, are in flight together
 constexpr int TAKE_SPAN = CP_THREADS * TAKE_PER;
@@ -912,6 +931,7 @@ struct TakeArgs {
     TakeTensor t[TAKE_MAX];
 };
 
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 template <typename V>
 __device__ __forceinline__ void take_block(const TakeTensor& t, uint32_t block, const int* __restrict__ ids) {
     const V* src = static_cast<const V*>(t.src);
@@ -930,10 +950,13 @@ __device__ __forceinline__ void take_block(const TakeTensor& t, uint32_t block, 
     }
     V v[TAKE_PER];
 #pragma unroll
-    for (int k = 0; k < TAKE_PER; ++k) v[k] = from[k] >= 0 ? src[from[k]] : V{};
+    for (int k = 0; k < TAKE_PER; ++k) v[k] = from[k] >= 0 ? __builtin_nontemporal_load(src + from[k]) : V{};
 #pragma unroll
     for (int k = 0; k < TAKE_PER; ++k)
-        if (to[k] >= 0) dst[to[k]] = v[k];
+        if (to[k] >= 0) {
+            if constexpr (sizeof(V) == 16) __builtin_nontemporal_store(v[k], dst + to[k]);
+            else dst[to[k]] = v[k];
+        }
     if (t.pad > 0 && block == t.blocks - 1) {  // the words behind the last row
         uint32_t* tail = reinterpret_cast<uint32_t*>(dst + (long long)t.K * t.t.units);
         for (int k = threadIdx.x; k < t.pad; k += CP_THREADS) tail[k] = 0u;
@@ -949,7 +972,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_take_rows(TakeArgs a, const int*
     }
     const TakeTensor t = a.t[lo];
     const uint32_t block = blockIdx.x - t.block0;
-    if (t.vec == 4) take_block<uint4>(t, block, ids);
+    if (t.vec == 4) take_block<u4v>(t, block, ids);
     else take_block<uint32_t>(t, block, ids);
 }
 
@@ -1040,10 +1063,15 @@ GSR_API int gsr_sh_colors_quantize(int P, int V, int degree, int M, const float*
     const ShArgs a = sh_args(P, V, M, xyz, nullptr, 0, nullptr, nullptr, campos);
     const unsigned grid = grid_for(P, 1LL << 31);
     hipStream_t st = (hipStream_t)stream;
-    if (degree == 0) k_sh_colors_quantize<0><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors);
-    else if (degree == 1) k_sh_colors_quantize<1><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors);
-    else if (degree == 2) k_sh_colors_quantize<2><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors);
-    else k_sh_colors_quantize<3><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors);
+    const bool nt = 12LL * M * P > NT_LOAD_BYTES;
+#define GSR_SH_QUANTIZE(D)                                                                                    \
+    if (nt) k_sh_colors_quantize<D, true><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors); \
+    else k_sh_colors_quantize<D, false><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors)
+    if (degree == 0) { GSR_SH_QUANTIZE(0); }
+    else if (degree == 1) { GSR_SH_QUANTIZE(1); }
+    else if (degree == 2) { GSR_SH_QUANTIZE(2); }
+    else { GSR_SH_QUANTIZE(3); }
+#undef GSR_SH_QUANTIZE
     return launched("sh_colors_quantize");
 }
 
@@ -1056,14 +1084,19 @@ GSR_API int gsr_sh_colors_backward(int P, int V, int degree, int M, const float*
     const ShArgs a = sh_args(P, V, M, xyz, nullptr, 0, codes, scales, campos);
     const unsigned grid = grid_for(P, 1LL << 31);
     hipStream_t st = (hipStream_t)stream;
-#define GSR_SH_BACKWARD(D)                                                                              \
-    if (dfeatures) k_sh_colors_backward<D, true><<<grid, CP_THREADS, 0, st>>>(a, mask, dcolors, dxyz, ddc, dfeatures); \
-    else k_sh_colors_backward<D, false><<<grid, CP_THREADS, 0, st>>>(a, mask, dcolors, dxyz, ddc, dfeatures)
+    const bool nt = 12LL * M * P > NT_STORE_BYTES;
+#define GSR_SH_BACKWARD_AS(...) \
+    k_sh_colors_backward<__VA_ARGS__><<<grid, CP_THREADS, 0, st>>>(a, mask, dcolors, dxyz, ddc, dfeatures)
+#define GSR_SH_BACKWARD(D)                              \
+    if (!dfeatures) GSR_SH_BACKWARD_AS(D, false, false); \
+    else if (nt) GSR_SH_BACKWARD_AS(D, true, true);      \
+    else GSR_SH_BACKWARD_AS(D, true, false)
     if (degree == 0) { GSR_SH_BACKWARD(0); }
     else if (degree == 1) { GSR_SH_BACKWARD(1); }
     else if (degree == 2) { GSR_SH_BACKWARD(2); }
     else { GSR_SH_BACKWARD(3); }
 #undef GSR_SH_BACKWARD
+#undef GSR_SH_BACKWARD_AS
     return launched("sh_colors_backward");
 }
 
