@@ -784,7 +784,7 @@ __global__ void __launch_bounds__(KEEP_SMALL_THREADS) k_keep_small(KeepArgs a, c
             }
         }
     }
-    for (int i = G.old_end + threadIdx.x; i < G.end; i += KEEP_SMALL_THREADS) ids[G.out + G.pick + (i - G.old_end)] = i;
+    for (int k = threadIdx.x; k < G.end - G.old_end; k += KEEP_SMALL_THREADS) ids[G.out + G.pick + k] = G.old_end + k;
 }
 
 __global__ void __launch_bounds__(CP_THREADS) k_keep_clear(uint32_t* __restrict__ p, int n) {
@@ -981,6 +981,9 @@ unsigned grid_for(long long items, long long cap) {
     return (unsigned)(g < 1 ? 1 : g > cap ? cap : g);
 }
 
+// One thread per Gaussian, its index an int: the last block's must not pass 2^31.
+constexpr int MAX_P = 0x7FFFFFFF - CP_THREADS;
+
 int check_rows(long long R, int K) {
     if (R < 0 || K < 0 || K > (1 << 20)) return set_error("[gsr] mx4: invalid number or width of rows");
     return 0;
@@ -988,7 +991,8 @@ int check_rows(long long R, int K) {
 
 int check_colors(int P, int V, int degree, int M, const float* xyz, const float* dc, const uint32_t* codes,
                  const uint8_t* scales, const float* campos) {
-    if (P < 0 || V < 1 || V > GSR_MAX_VIEWS) return set_error("[gsr] sh_colors: invalid P or number of views");
+    if (P < 0 || P > MAX_P || V < 1 || V > GSR_MAX_VIEWS)
+        return set_error("[gsr] sh_colors: invalid P or number of views");
     if (degree < 0 || degree > 3 || M < (degree + 1) * (degree + 1) || M > 16)
         return set_error("[gsr] sh_colors: degree must be 0..3 with (degree + 1)^2 <= M <= 16");
     if (P > 0 && (!xyz || !dc || !campos || (M > 1 && (!codes || !scales))))
@@ -1102,7 +1106,7 @@ GSR_API int gsr_sh_colors_backward(int P, int V, int degree, int M, const float*
 
 GSR_API int gsr_accumulate_weights(int P, const float* weights, long long stride, float decay, float* acc,
                                    void* stream) {
-    if (P < 0) return set_error("[gsr] gsr_accumulate_weights: P < 0");
+    if (P < 0 || P > MAX_P) return set_error("[gsr] gsr_accumulate_weights: invalid P");
     if (P == 0) return 0;
     if (!weights || !acc) return set_error("[gsr] gsr_accumulate_weights: null buffer");
     k_accumulate_weights<<<grid_for(P, 1LL << 31), CP_THREADS, 0, (hipStream_t)stream>>>(P, weights, stride, decay, acc);
@@ -1163,6 +1167,24 @@ GSR_API int gsr_take_rows(int K, const int* ids, int n, const gsr_rows* tensors,
         const long long words = (long long)K * t.width;
         if ((words > 0 && t.rows > 0 && !t.src) || (words + t.pad > 0 && !t.dst))
             return set_error("[gsr] gsr_take_rows: null buffer");
+    }
+    // what is written is neither read nor written by another tensor of the call
+    struct Range {
+        uintptr_t lo, hi;
+        bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
+    };
+    auto written = [&](const gsr_rows& t) -> Range {
+        return {(uintptr_t)t.dst, (uintptr_t)t.dst + 4 * ((uintptr_t)K * t.width + t.pad)};
+    };
+    for (int k = 0; k < n; ++k) {
+        const Range w = written(tensors[k]);
+        bool clash = w.meets({(uintptr_t)ids, (uintptr_t)ids + 4 * (uintptr_t)K});
+        for (int j = 0; j < n; ++j) {
+            const gsr_rows& t = tensors[j];
+            clash |= w.meets({(uintptr_t)t.src, (uintptr_t)t.src + 4 * (uintptr_t)t.rows * t.width});
+            clash |= j != k && w.meets(written(t));
+        }
+        if (clash) return set_error("[gsr] gsr_take_rows: a destination overlaps the ids or another tensor of the call");
     }
     hipStream_t st = (hipStream_t)stream;
     bool any = false;

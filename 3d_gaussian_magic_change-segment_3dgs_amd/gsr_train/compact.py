@@ -258,8 +258,10 @@ def sh_colors(xyz, features_dc, rest, campos, degree):
 
     xyz [P, 3], features_dc [P, 1, 3] or [P, 3], rest an MX4Rows of P rows of 3 (M - 1)
     values, campos [3] -> colors [P, 3], or [V, 3] -> [V, P, 3].  Differentiable in xyz and
-    features_dc (gradients summed over the views); a channel that the clamp holds at zero
-    gives no gradient, and a Gaussian at the camera position itself none to xyz."""
+    features_dc (gradients summed over the views; campos gets none, nor do the codes); a
+    channel that the clamp holds at zero gives no gradient, and a Gaussian at the camera
+    position itself none to xyz.  A features_dc of its own ([P, 3] contiguous) is read faster
+    than a view of [P, M, 3] features, whose rows lie a cache line apart."""
     if _HOST is not None and isinstance(rest, MX4Rows) and _plain(xyz, features_dc, campos, degree):
         return _HOST.sh_colors(xyz, features_dc, rest.codes, rest.scales, rest.width, campos, degree)
     if not isinstance(rest, MX4Rows) or rest.width % 3 or rest.width > 45:
@@ -457,7 +459,7 @@ class CompactGaussians:
     @property
     def get_features(self):
         """Decoded coefficients, float32 [P, M, 3]."""
-        return torch.cat((self.features_dc, self.rest.dequantize().view(self.num_points, -1, 3)), 1)
+        return torch.cat((self.features_dc, self.rest.dequantize().view(self.num_points, self.rest.width // 3, 3)), 1)
 
     @torch.no_grad()
     def get_colors(self, campos):

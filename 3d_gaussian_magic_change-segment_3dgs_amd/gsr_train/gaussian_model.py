@@ -113,7 +113,7 @@ class GaussianModel:
         self.optimizer = None
         self.percent_dense = 0
         self.spatial_lr_scale = 0
-        self.feature_bits = 32  # 4: get_colors rounds the SH coefficients as compact() stores them
+        self.feature_bits = 32
         self._allocate(0)
 
     # ---- storage ------------------------------------------------------------------------
@@ -151,6 +151,17 @@ class GaussianModel:
     _segment = property(lambda self: self.group_view("segment"))
     _scaling = property(lambda self: self.group_view("scaling"))
     _rotation = property(lambda self: self.group_view("rotation"))
+
+    @property
+    def feature_bits(self):
+        """32, or 4: render with get_colors, the SH coefficients as compact() stores them."""
+        return self._feature_bits
+
+    @feature_bits.setter
+    def feature_bits(self, bits):
+        if bits not in (4, 32):
+            raise ValueError(f"GaussianModel: feature_bits must be 4 or 32 (got {bits!r})")
+        self._feature_bits = bits
 
     @property
     def num_points(self):
@@ -427,10 +438,9 @@ class GaussianModel:
     def compact(self):
         """The scene as it is rendered, with the SH coefficients above the constant one in 4
         bits and no training state (CompactGaussians)."""
-        P = self.num_points
         features = self.get_features
         return _compact.CompactGaussians(
-            self.get_xyz.clone(), features[:, :1].clone(), _compact.mx4_quantize(features.view(P, -1)[:, 3:]),
+            self.get_xyz.clone(), features[:, :1].clone(), _compact.mx4_quantize(features.flatten(1)[:, 3:]),
             self.get_opacity.clone(), self.get_scaling.clone(), self.get_rotation.clone(), self.get_segment.clone(),
             self.active_sh_degree)
 

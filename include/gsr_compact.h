@@ -85,7 +85,8 @@ GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const g
 
 /* dst[j] = src[ids[j]], j < K, for n tensors of rows of `width` 32-bit words.  An id
  * outside [0, rows) gives a row of zeros.  `pad` words behind a destination's last row
- * are cleared too (the padding of an arena block). */
+ * are cleared too (the padding of an arena block).  A destination that overlaps the ids or
+ * another tensor of the call is refused. */
 typedef struct gsr_rows {
     const void* src;
     void* dst;

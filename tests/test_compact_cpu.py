@@ -56,6 +56,14 @@ def test_c_calls_validate_without_the_device():
     assert L.gsr_take_rows(3, 16, 1, (T._Rows * 1)((16, None, 3, 5, 0)), None) != 0 and "null buffer" in err()
     assert L.gsr_take_rows(3, 16, 1, (T._Rows * 1)((16, 16, -3, 5, 0)), None) != 0
     assert L.gsr_take_rows(0, None, 1, (T._Rows * 1)((16, None, 3, 5, 0)), None) == 0
+    # what is written overlaps: the source, the ids, another source, another destination, by its padding alone
+    a, b, c, d = 0x10000, 0x20000, 0x30000, 0x40000
+    for bad in ([(a, a, 3, 5, 0)], [(a, a + 48, 3, 5, 0)], [(a, d, 3, 5, 0)], [(a, b, 3, 5, 0), (b + 32, c, 3, 5, 0)],
+                [(a, c, 3, 5, 0), (b, c + 32, 3, 5, 0)], [(a, b - 36, 3, 5, 1), (b, c, 3, 5, 0)]):
+        assert L.gsr_take_rows(3, d, len(bad), (T._Rows * len(bad))(*bad), None) != 0 and "overlaps" in err()
+    big = 2 ** 31 - 1
+    assert L.gsr_sh_colors(big, 1, 0, 1, 16, 16, 3, None, None, 16, 16, None, None) != 0
+    assert L.gsr_accumulate_weights(big, 16, 1, 1.0, 16, None) != 0
 
 
 def refused(fn, *a, match, **k):
@@ -126,6 +134,15 @@ def test_python_refusals(route, monkeypatch):
     refused(G.take_rows, ids, [z(4, 3)], out=[], match="one output")
     refused(G.accumulate_weights, w, z(9), match="shape")
     refused(G.accumulate_weights, w, w, match="GPU")
+
+
+def test_feature_bits_are_4_or_32():
+    from gsr_train import GaussianModel
+    m = GaussianModel(1, device="cpu")
+    assert m.feature_bits == 32
+    m.feature_bits = 4
+    with pytest.raises(ValueError, match="4 or 32"):
+        m.feature_bits = 8
 
 
 def test_keep_groups_cut_to_what_a_group_holds():

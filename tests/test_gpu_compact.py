@@ -411,6 +411,17 @@ def test_take_rows(K):
     assert all(torch.equal(a, b) for a, b in zip(out, got))
 
 
+def test_take_rows_refuses_an_output_that_overlaps(monkeypatch):
+    import gsr_train as G
+    x = torch.randn(10, 3, device=DEV)
+    ids = torch.arange(10, dtype=torch.int32, device=DEV)
+    for _ in both_routes(monkeypatch):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            G.take_rows(ids, [x], out=[x])
+        with pytest.raises(RuntimeError, match="overlaps"):
+            G.take_rows(ids, [x, x.clone()], out=[torch.empty_like(x), x])
+
+
 def test_take_rows_of_ids_outside():
     import gsr_train as G
     x = torch.randn(10, 3, device=DEV)
@@ -579,6 +590,85 @@ def test_sh0_model_has_no_codes():
         b = render(cam, m, bg)["render"]
         c = render(cam, m.compact(), bg)["render"]
     assert torch.equal(b, c) and torch.allclose(a, b, atol=1e-5)
+
+
+def test_models_without_gaussians_or_optimizer():
+    from gsr_train import GaussianModel
+    for degree in (0, 3):
+        e = GaussianModel(degree, device=DEV)
+        e.feature_bits = 4
+        small = e.compact()
+        cam = torch.zeros(3, device=DEV)
+        assert small.num_points == 0 and small.get_features.shape == (0, (degree + 1) ** 2, 3)
+        assert small.get_colors(cam).shape == (0, 3) and e.get_colors(cam).shape == (0, 3)
+        ids, ranges = e.evict(5)
+        assert ids.numel() == 0 and ranges == [(0, 0)] and e.num_points == 0
+    m = model(degree=1)
+    m.optimizer = None  # a scene that was only loaded
+    want = O.keep_heaviest(m.contribution.cpu().numpy().reshape(-1), [(0, 3000, 100, 10)])
+    xyz = m._xyz.clone()
+    ids, _ = m.evict(100, recent=10)
+    assert np.array_equal(ids.cpu().numpy(), want) and torch.equal(m._xyz, xyz[ids.long()])
+    m2 = model(degree=0)
+    assert m2.compact().get_features.shape == (3000, 1, 3)
+
+
+def test_step_after_eviction():
+    """The optimizer goes on with the moments of the Gaussians that stayed."""
+    a, b = model(), model()
+    ids, _ = a.evict(1200)
+    g = torch.randn(a._spec.total, generator=gen(4)).to(DEV)
+    full = torch.zeros(b._spec.total, device=DEV)
+    for name in ("xyz", "features", "opacity", "scaling", "rotation", "segment"):
+        b._spec.block(full, name)[ids.long()] = a._spec.block(g, name)
+    for m, grad in ((a, g), (b, full)):
+        m._arena.grad = grad
+        m.optimizer.step()
+    for name in ("xyz", "features", "opacity", "scaling", "rotation", "segment"):
+        assert torch.equal(a._spec.block(a._arena.data, name), b._spec.block(b._arena.data, name)[ids.long()]), name
+
+
+# ---- offsets past 32 bits --------------------------------------------------------------------------
+def test_offsets_past_32_bits():
+    """45M Gaussians at degree 3: 2.16e9 feature values, 8.6 GB.  All zero but for the last rows and a few
+    others, which have to come out as in a tensor of their own."""
+    import gsr_train as G
+    P, tail = 45_000_000, 300
+    some = torch.cat([torch.arange(50), torch.arange(22_369_600, 22_369_700), torch.arange(P - tail, P)])
+    xyz, f, cam, up = scene(len(some), 16, 1, 31)
+    at = some.to(DEV)
+    x = torch.zeros(P, 3, device=DEV)
+    x[at] = xyz.to(DEV)
+    feat = torch.zeros(P, 16, 3, device=DEV)
+    feat[at] = f.to(DEV)
+    q, want = G.mx4_quantize(feat.flatten(1)[:, 3:]), G.mx4_quantize(f.to(DEV).flatten(1)[:, 3:])
+    assert torch.equal(q.codes[at], want.codes) and torch.equal(q.scales[at], want.scales)
+    assert int(q.codes.ne(0).any(1).sum()) == int(want.codes.ne(0).any(1).sum())
+    back = q.dequantize()
+    assert torch.equal(back[at], want.dequantize())
+    del back
+    x.requires_grad_()
+    feat.requires_grad_()
+    sx, sf = xyz.to(DEV).requires_grad_(), f.to(DEV).requires_grad_()
+    c, s = G.sh_colors_quantized(x, feat, cam[0].to(DEV), 3), G.sh_colors_quantized(sx, sf, cam[0].to(DEV), 3)
+    assert torch.equal(c[at], s)
+    assert torch.equal(G.sh_colors(x.detach(), feat.detach()[:, 0], q, cam[0].to(DEV), 3)[at], s)
+    g = torch.zeros(P, 3, device=DEV)
+    g[at] = up[0].to(DEV)
+    gx, gf = torch.autograd.grad(c, (x, feat), g)
+    hx, hf = torch.autograd.grad(s, (sx, sf), up[0].to(DEV))
+    assert torch.equal(gx[at], hx) and torch.equal(gf[at], hf)
+    assert int(gf.flatten(1).ne(0).any(1).sum()) == int(hf.flatten(1).ne(0).any(1).sum())
+    del c, gx, gf, g, q
+    w = torch.zeros(P, device=DEV)
+    w[at] = torch.rand(len(some), generator=gen(2)).to(DEV) + 1
+    ids = G.keep_heaviest(w, len(some))
+    assert torch.equal(ids.cpu().long(), some)
+    # many rows out: the kept ones and everything behind the first 100
+    ids = torch.arange(100, P, dtype=torch.int32, device=DEV)
+    (rows,) = G.take_rows(ids, [feat.detach()])
+    assert torch.equal(rows[-tail:], f[-tail:].to(DEV)) and int(rows[:1000].ne(0).sum()) == 0
+    assert torch.equal(rows[22_369_500:22_369_600], f[50:150].to(DEV))
 
 
 # ---- graphs --------------------------------------------------------------------------------------
