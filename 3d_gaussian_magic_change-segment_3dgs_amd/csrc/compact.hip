@@ -305,9 +305,12 @@ __device__ __forceinline__ float normalize3(float& x, float& y, float& z) {
         x /= m; y /= m; z /= m;
         n = mad(x, x, mad(y, y, z * z));
     }
-    const float r = 1.0f / sqrtf(n);
+    // the hardware's reciprocal root (good to 2 units of 2^-24) and a Newton step: a third of the
+    // instructions of a rounded root and quotient
+    float r = __builtin_amdgcn_rsqf(n);
+    r *= mad(-0.5f * n * r, r, 1.5f);
     x *= r; y *= r; z *= r;
-    return r / m;
+    return m == 1.0f ? r : r / m;
 }
 
 // The value before the clamp in 64 bits.
