@@ -10,6 +10,8 @@ plus the sum over at most 16 views: 2^-18 sum |g|.  Gradients of the positions: 
 gradient (length at most 3.5, slope at most 15) is off by 6 * 15 + 8 * 3.5 u, the weights
 (3 products) and their sum over 16 by 19 * 3.5 u, the projection and 1 / |u| by 6 * 3.5 u:
 about 205 u < 2^-16 times sum_v 1 / |u_v| sum |coefficient| |g|."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -44,6 +46,19 @@ def test_mx4_rows(R, K):
     g = gen(R * 1000 + K)
     x = torch.randn(R, K, generator=g) * torch.exp(torch.randn(R, 1, generator=g) * 3)
     x[:: 5] = 0.0
+    check_rows(x.to(DEV), f"{R}x{K}")
+
+
+@pytest.mark.parametrize("R,K", [(1, 4), (2, 5), (3, 35), (1000, 9), (700, 45), (3, 1024), (7, 1025), (5, 1029), (11, 5000),
+                                 (300, 34), (2049, 6), (91, 31), (40, 63)])
+def test_mx4_rows_of_any_width_with_holes(R, K):
+    """Rows and blocks that end inside a lane's four values; NaN and infinities here and there: only their own blocks
+    read back as NaN."""
+    g = gen(R * 7919 + K)
+    x = torch.randn(R, K, generator=g) * torch.exp(torch.randn(R, 1, generator=g) * 3)
+    hole = torch.rand(R, K, generator=g)
+    x[hole < 0.01] = math.nan
+    x[hole > 0.995] = -math.inf
     check_rows(x.to(DEV), f"{R}x{K}")
 
 
