@@ -220,71 +220,71 @@ __device__ __forceinline__ float mad(float a, float b, float c) { return __built
 __device__ __forceinline__ double mad(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
 // Real spherical harmonics up to degree 3 in the reference's order and signs
-// (utils/sh_utils.py:26-48); F = float, or double where a sign needs it.
+// (utils/sh_utils.py:26-48): Y_k = SH_C[k] p_k(x, y, z), p_k the polynomials of sh_values.  The
+// constants go into a Gaussian's coefficients once, not into every view's basis (8 views of 300k
+// Gaussians at degree 3: 11.6 -> 10.7 us).
+__device__ constexpr double SH_C[16] = {
+    0.28209479177387814,
+    -0.4886025119029199, 0.4886025119029199, -0.4886025119029199,
+    1.0925484305920792, -1.0925484305920792, 0.31539156525252005, -1.0925484305920792, 0.5462742152960396,
+    -0.5900435899266435, 2.890611442640554, -0.4570457994644658, 0.3731763325901154, -0.4570457994644658,
+    1.445305721320277, -0.5900435899266435};
+
+// p_k, k >= 1 (p_0 = 1); F = float, or double where a sign needs it.
 template <int DEG, typename F>
 __device__ __forceinline__ void sh_values(F x, F y, F z, F* b) {
-    b[0] = (F)0.28209479177387814;
+    b[0] = (F)1;
     if constexpr (DEG > 0) {
-        const F c1 = (F)0.4886025119029199;
-        b[1] = -c1 * y; b[2] = c1 * z; b[3] = -c1 * x;
+        b[1] = y; b[2] = z; b[3] = x;
     }
     if constexpr (DEG > 1) {
-        const F a = (F)1.0925484305920792, c = (F)0.31539156525252005, e = (F)0.5462742152960396;
-        const F xx = x * x, yy = y * y, zz = z * z, t = xx + yy, d = xx - yy;
-        b[4] = a * (x * y); b[5] = -a * (y * z); b[6] = c * mad((F)2, zz, -t); b[7] = -a * (x * z);
-        b[8] = e * d;
+        const F xx = x * x, yy = y * y, zz2 = (F)2 * (z * z), t = xx + yy, d = xx - yy;
+        b[4] = x * y; b[5] = y * z; b[6] = zz2 - t; b[7] = x * z;
+        b[8] = d;
         if constexpr (DEG > 2) {
-            const F p = (F)0.5900435899266435, q = (F)2.890611442640554, r = (F)0.4570457994644658,
-                    s = (F)0.3731763325901154, u = (F)1.445305721320277;
-            const F o = -r * mad((F)4, zz, -t);
-            b[9] = -p * y * mad((F)3, xx, -yy);
-            b[10] = q * (x * y) * z;
+            const F o = mad((F)2, zz2, -t);
+            b[9] = y * mad((F)3, xx, -yy);
+            b[10] = b[4] * z;
             b[11] = o * y;
-            b[12] = s * z * mad((F)2, zz, (F)-3 * t);
+            b[12] = z * mad((F)-3, t, zz2);
             b[13] = o * x;
-            b[14] = u * z * d;
-            b[15] = -p * x * mad((F)-3, yy, xx);
+            b[14] = z * d;
+            b[15] = x * mad((F)-3, yy, xx);
         }
     }
 }
 
-// sum_k w[k] grad Y_k at (x, y, z) (gradients of the polynomials above; what they have along
-// (x, y, z) itself drops out in the projection that follows).
+// sum_k w[k] grad p_k at (x, y, z) (what they have along (x, y, z) itself drops out in the
+// projection that follows).
 template <int DEG>
 __device__ __forceinline__ void sh_grad(float x, float y, float z, const float* w, float& gx, float& gy, float& gz) {
     gx = gy = gz = 0.0f;
     if constexpr (DEG > 0) {
-        const float c1 = 0.4886025119029199f;
-        gx = -c1 * w[3]; gy = -c1 * w[1]; gz = c1 * w[2];
+        gx = w[3]; gy = w[1]; gz = w[2];
     }
     if constexpr (DEG > 1) {
-        const float a = 1.0925484305920792f, c = 0.31539156525252005f, e = 0.5462742152960396f;
-        const float w4 = a * w[4], w5 = -a * w[5], w6 = 2.0f * c * w[6], w7 = -a * w[7], w8 = 2.0f * e * w[8];
-        gx = mad(y, w4, mad(z, w7, mad(x, w8 - w6, gx)));
-        gy = mad(x, w4, mad(z, w5, mad(-y, w8 + w6, gy)));
-        gz = mad(y, w5, mad(x, w7, mad(2.0f * z, w6, gz)));
+        const float w6 = 2.0f * w[6], w8 = 2.0f * w[8];
+        gx = mad(y, w[4], mad(z, w[7], mad(x, w8 - w6, gx)));
+        gy = mad(x, w[4], mad(z, w[5], mad(-y, w8 + w6, gy)));
+        gz = mad(y, w[5], mad(x, w[7], mad(2.0f * z, w6, gz)));
     }
     if constexpr (DEG > 2) {
-        const float p = 0.5900435899266435f, q = 2.890611442640554f, r = 0.4570457994644658f,
-                    s = 0.3731763325901154f, u = 1.445305721320277f;
         const float xx = x * x, yy = y * y, zz = z * z, xy = x * y, yz = y * z, xz = x * z, t = xx + yy, d = xx - yy;
-        const float w9 = 3.0f * p * w[9], w10 = q * w[10], w11 = r * w[11], w12 = 3.0f * s * w[12],
-                    w13 = r * w[13], w14 = u * w[14], w15 = 3.0f * p * w[15];
-        const float z4 = 4.0f * zz;
-        gx = mad(-2.0f * xy, w9 - w11, gx);
-        gx = mad(yz, w10, gx);
-        gx = mad(2.0f * xz, w14 - w12, gx);
-        gx = mad(-(z4 - mad(2.0f, xx, t)), w13, gx);
-        gx = mad(-d, w15, gx);
-        gy = mad(-d, w9, gy);
-        gy = mad(xz, w10, gy);
-        gy = mad(-(z4 - mad(2.0f, yy, t)), w11, gy);
-        gy = mad(-2.0f * yz, w12 + w14, gy);
-        gy = mad(2.0f * xy, w13 + w15, gy);
-        gz = mad(xy, w10, gz);
-        gz = mad(-8.0f * z, mad(y, w11, x * w13), gz);
+        const float w9 = 3.0f * w[9], w12 = 3.0f * w[12], w15 = 3.0f * w[15], z4 = 4.0f * zz;
+        gx = mad(2.0f * xy, w9 - w[11], gx);
+        gx = mad(yz, w[10], gx);
+        gx = mad(2.0f * xz, w[14] - w12, gx);
+        gx = mad(z4 - mad(2.0f, xx, t), w[13], gx);
+        gx = mad(d, w15, gx);
+        gy = mad(d, w9, gy);
+        gy = mad(xz, w[10], gy);
+        gy = mad(z4 - mad(2.0f, yy, t), w[11], gy);
+        gy = mad(-2.0f * yz, w12 + w[14], gy);
+        gy = mad(-2.0f * xy, w[13] + w15, gy);
+        gz = mad(xy, w[10], gz);
+        gz = mad(8.0f * z, mad(y, w[11], x * w[13]), gz);
         gz = mad(mad(2.0f, zz, -t), w12, gz);
-        gz = mad(d, w14, gz);
+        gz = mad(d, w[14], gz);
     }
 }
 
@@ -305,67 +305,100 @@ __device__ __forceinline__ v3a load3(const float* p) { return {p[0], p[1], p[2]}
 __device__ __forceinline__ void store3(float* p, float x, float y, float z) {
     p[0] = x; p[1] = y; p[2] = z;
 }
+__device__ __forceinline__ void store3_past(float* p, float x, float y, float z) {  // past the caches
+    __builtin_nontemporal_store(x, p);
+    __builtin_nontemporal_store(y, p + 1);
+    __builtin_nontemporal_store(z, p + 2);
+}
 
-// Decoded coefficients of one Gaussian, 3 floats each, coefficient 0 the constant one.
+// Coefficients of one Gaussian, 3 floats each, coefficient 0 the constant one: decoded, then times
+// SH_C (fold).  The codes stay for the sign in 64 bits.
 template <int DEG>
 struct Coef {
     static constexpr int N = (DEG + 1) * (DEG + 1);
     static constexpr int WORDS = (3 * (N - 1) + 7) / 8;   // code words that the degree needs
     static constexpr int BLOCKS = (3 * (N - 1) + GSR_MX_BLOCK - 1) / GSR_MX_BLOCK;
-    float q[8 * WORDS + 3];
+    float q[8 * WORDS + 3];   // q[0..2] as they are
+    float base[3];            // 1/2 + Y_0 dc
+    uint32_t w[WORDS + 1];
+    uint32_t bytes;           // scales
+    __device__ __forceinline__ float scale(int block) const { return mx_scale(bytes >> (8 * block) & 255u); }
+    __device__ __forceinline__ void decode() {
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) mx_decode8(w[j], scale(j / 4), q + 3 + 8 * j);
+    }
+    __device__ __forceinline__ void fold() {
+#pragma unroll
+        for (int j = 0; j < 3; ++j) base[j] = mad((float)SH_C[0], q[j], 0.5f);
+#pragma unroll
+        for (int k = 1; k < N; ++k)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) q[3 * k + j] *= (float)SH_C[k];
+    }
     __device__ __forceinline__ void load(int i, const ShArgs& a) {
         const v3a d = a.dc ? load3(a.dc + i * a.dc_stride) : v3a{0.0f, 0.0f, 0.0f};
         q[0] = d.x; q[1] = d.y; q[2] = d.z;
-        uint32_t w[WORDS + 1];
 #pragma unroll
         for (int k = 0; k < WORDS; ++k) w[k] = a.codes[(long long)i * a.pitch + k];
+        bytes = 0;
 #pragma unroll
-        for (int k = 0; k < BLOCKS; ++k) {
-            const float scale = mx_scale(a.scales[(long long)i * a.nb + k]);
-#pragma unroll
-            for (int j = 4 * k; j < 4 * k + 4; ++j)
-                if (j < WORDS) mx_decode8(w[j], scale, q + 3 + 8 * j);
-        }
+        for (int k = 0; k < BLOCKS; ++k) bytes |= (uint32_t)a.scales[(long long)i * a.nb + k] << (8 * k);
+        decode();
     }
-    // The value before the clamp for basis values b: smallest terms first.
-    template <typename F>
-    __device__ __forceinline__ void sum(const F* b, F* s) const {
+    // The value before the clamp for basis polynomials b: smallest terms first.
+    __device__ __forceinline__ void sum(const float* b, float* s) const {
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
-            F t = 0;
+            float t = 0.0f;
 #pragma unroll
-            for (int k = N - 1; k >= 0; --k) t = mad(b[k], (F)q[3 * k + j], t);
-            s[j] = t + (F)0.5;
+            for (int k = N - 1; k >= 1; --k) t = mad(b[k], q[3 * k + j], t);
+            s[j] = t + base[j];
         }
     }
 };
 
 // u -> u / |u|; returns 1 / |u|, 0 (and d = 0) where u is 0.
 __device__ __forceinline__ float normalize3(float& x, float& y, float& z) {
-    float n = mad(x, x, mad(y, y, z * z)), m = 1.0f;
-    if (!(n > 1e-30f && n < 1e30f)) {  // the squares leave the range (or u is 0, or not finite)
-        m = fmaxf(fabsf(x), fmaxf(fabsf(y), fabsf(z)));
-        if (!(m > 0.0f)) return 0.0f;
-        x /= m; y /= m; z /= m;
-        n = mad(x, x, mad(y, y, z * z));
+    float n = mad(x, x, mad(y, y, z * z)), back = 1.0f;
+    if (__builtin_expect(!(n > 1e-30f && n < 1e30f), 0)) {  // the squares leave the range (or u is 0, or not finite)
+        const float m = fmaxf(fabsf(x), fmaxf(fabsf(y), fabsf(z)));
+        const bool some = m > 0.0f;
+        const float by = some ? m : 1.0f;
+        x /= by; y /= by; z /= by;
+        n = some ? mad(x, x, mad(y, y, z * z)) : 1.0f;
+        back = some ? 1.0f / m : 0.0f;
     }
     // the hardware's reciprocal root (good to 2 units of 2^-24) and a Newton step: a third of the
     // instructions of a rounded root and quotient
     float r = __builtin_amdgcn_rsqf(n);
     r *= mad(-0.5f * n * r, r, 1.5f);
     x *= r; y *= r; z *= r;
-    return m == 1.0f ? r : r / m;
+    return r * back;
 }
 
-// The value before the clamp in 64 bits.
+// The value before the clamp in 64 bits, from the codes.
 template <int DEG>
-__device__ __forceinline__ void preclamp64(const Coef<DEG>& c, v3a p, const float* cam, double* s) {
-    const double x = (double)p.x - cam[0], y = (double)p.y - cam[1], z = (double)p.z - cam[2];
+__device__ __forceinline__ void preclamp64(const Coef<DEG>& c, v3a p, float cx, float cy, float cz, double* s) {
+    constexpr int N = Coef<DEG>::N;
+    const double x = (double)p.x - cx, y = (double)p.y - cy, z = (double)p.z - cz;
     const double n = x * x + y * y + z * z;
     const double r = n > 0.0 ? 1.0 / sqrt(n) : 0.0;
-    double b[Coef<DEG>::N];
+    double b[N];
     sh_values<DEG, double>(x * r, y * r, z * r, b);
-    c.template sum<double>(b, s);
+#pragma unroll
+    for (int j = 0; j < 3; ++j) s[j] = mad(SH_C[0], (double)c.q[j], 0.5);
+#pragma unroll
+    for (int m = 0; m < Coef<DEG>::WORDS; ++m) {
+        float v[8];
+        uint32_t w = c.w[m];
+        asm volatile("" : "+v"(w));  // decoded here, not kept in registers through the views
+        mx_decode8(w, c.scale(m / 4), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int f = 8 * m + e + 3, k = f / 3;
+            if (k < N) s[f % 3] = mad(SH_C[k] * b[k], (double)v[e], s[f % 3]);
+        }
+    }
 }
 
 // Colours of one Gaussian in every view; with MASK, which channels the clamp lets through (a
@@ -373,8 +406,8 @@ __device__ __forceinline__ void preclamp64(const Coef<DEG>& c, v3a p, const floa
 // 6, a basis value (slope at most 4.9) to 37, the sum of 16 products to 53 of the coefficients'
 // sum; nearer to zero than 64 the sign is taken from 64 bits, so that no gradient hangs on a
 // rounding.
-template <int DEG, bool MASK>
-__device__ __forceinline__ void write_colors(const ShArgs& a, int i, v3a p, const Coef<DEG>& c,
+template <int DEG, bool MASK, bool NT>
+__device__ __forceinline__ void write_colors(const ShArgs& a, int i, v3a p, Coef<DEG>& c,
                                              float* __restrict__ colors, uint8_t* __restrict__ mask) {
     float near[3] = {0.5f, 0.5f, 0.5f};
     if constexpr (MASK) {
@@ -385,9 +418,12 @@ __device__ __forceinline__ void write_colors(const ShArgs& a, int i, v3a p, cons
     }
 #pragma unroll
     for (int j = 0; j < 3; ++j) near[j] *= 0x1p-18f;
+    c.fold();
+    float cx = a.campos[0], cy = a.campos[1], cz = a.campos[2];
     for (int v = 0; v < a.V; ++v) {
-        const float* cam = a.campos + 3 * v;
-        float x = p.x - cam[0], y = p.y - cam[1], z = p.z - cam[2];
+        const float* ahead = a.campos + (v + 1 < a.V ? 3 * v + 3 : 0);  // the next camera, while this one's colours are made
+        const float nx = ahead[0], ny = ahead[1], nz = ahead[2];
+        float x = p.x - cx, y = p.y - cy, z = p.z - cz;
         normalize3(x, y, z);
         float b[Coef<DEG>::N], s[3];
         sh_values<DEG, float>(x, y, z, b);
@@ -401,7 +437,7 @@ __device__ __forceinline__ void write_colors(const ShArgs& a, int i, v3a p, cons
             }
             if (close) {
                 double t[3];
-                preclamp64<DEG>(c, p, cam, t);
+                preclamp64<DEG>(c, p, cx, cy, cz, t);
 #pragma unroll
                 for (int j = 0; j < 3; ++j) on[j] = t[j] >= 0.0;
             }
@@ -409,13 +445,22 @@ __device__ __forceinline__ void write_colors(const ShArgs& a, int i, v3a p, cons
         }
 #pragma unroll
         for (int j = 0; j < 3; ++j) s[j] = s[j] < 0.0f ? 0.0f : s[j];  // keeps a NaN
-        store3(colors + ((long long)v * a.P + i) * 3, s[0], s[1], s[2]);
+        float* o = colors + ((long long)v * a.P + i) * 3;
+        if constexpr (NT) store3_past(o, s[0], s[1], s[2]);
+        else store3(o, s[0], s[1], s[2]);
+        cx = nx; cy = ny; cz = nz;
     }
 }
 
+// Colours that do not fit the caches beside the inputs pass by them (write-back of their lines
+// stands in the way of reads, the next kernel's too): 28.8 MB (300k Gaussians, 8 views) 10.7 -> 9.3 us, 72 MB (6M,
+// one view) 65.7 -> 62.6, 48 MB in a training step of 1M with 4 views 111 -> 96; 12 MB (1M, one view) 10.5 -> 10.6.
+// (The same for reading their gradients: backward 48 -> 62 us, so not there.)
+constexpr long long NT_COLOR_BYTES = 16LL << 20;
+
 // One thread per Gaussian, its coefficients in registers for all views.  Bound by memory with
 // one view (62 bytes a Gaussian at degree 3), by the vector units with many.
-template <int DEG, bool MASK>
+template <int DEG, bool MASK, bool NT>
 __global__ void __launch_bounds__(CP_THREADS) k_sh_colors(ShArgs a, float* __restrict__ colors,
                                                           uint8_t* __restrict__ mask) {
     const int i = blockIdx.x * CP_THREADS + threadIdx.x;
@@ -423,7 +468,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors(ShArgs a, float* __res
     const v3a p = load3(a.xyz + 3LL * i);
     Coef<DEG> c;
     c.load(i, a);
-    write_colors<DEG, MASK>(a, i, p, c, colors, mask);
+    write_colors<DEG, MASK, NT>(a, i, p, c, colors, mask);
 }
 
 // ---- rows of features through LDS ------------------------------------------------
@@ -504,7 +549,7 @@ __device__ __forceinline__ void rows_out(float* __restrict__ dst, int rows, int 
 // Training forward: a Gaussian's fp32 coefficients are read once, rounded to codes (kept for the
 // backward), read back and evaluated.  The blocks that the degree touches are rounded whole, so a
 // code does not depend on the degree.
-template <int DEG, bool NT>
+template <int DEG, bool NT, bool NT_COLOR>
 __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, const float* __restrict__ features,
                                                                    uint32_t* __restrict__ codes,
                                                                    uint8_t* __restrict__ scales,
@@ -539,7 +584,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, con
     const v3a p = load3(a.xyz + 3LL * i);
     C c;
     c.q[0] = v[0]; c.q[1] = v[1]; c.q[2] = v[2];
-    uint32_t w[C::WORDS + 1], bytes = 0;
+    c.bytes = 0;
 #pragma unroll
     for (int b = 0; b < C::BLOCKS; ++b) {
         uint32_t m = 0;
@@ -549,21 +594,21 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, con
             m = m > x ? m : x;
         }
         const uint32_t sb = mx_scale_byte(m);
-        bytes |= sb << (8 * b);
+        c.bytes |= sb << (8 * b);
 #pragma unroll
         for (int j = 4 * b; j < 4 * b + 4; ++j)
             if (j < C::WORDS) {
                 const float* x = v + 3 + 8 * j;
-                w[j] = sb == 255u ? 0u : mx_encode8(v4a{x[0], x[1], x[2], x[3]}, v4a{x[4], x[5], x[6], x[7]},
-                                                    mx_scale(sb));
-                mx_decode8(w[j], mx_scale(sb), c.q + 3 + 8 * j);
+                c.w[j] = sb == 255u ? 0u : mx_encode8(v4a{x[0], x[1], x[2], x[3]}, v4a{x[4], x[5], x[6], x[7]},
+                                                      mx_scale(sb));
             }
     }
+    c.decode();
 #pragma unroll
-    for (int j = 0; j < C::WORDS; ++j) codes[(long long)i * a.pitch + j] = w[j];
+    for (int j = 0; j < C::WORDS; ++j) codes[(long long)i * a.pitch + j] = c.w[j];
 #pragma unroll
-    for (int b = 0; b < C::BLOCKS; ++b) scales[(long long)i * a.nb + b] = (uint8_t)(bytes >> (8 * b));
-    write_colors<DEG, true>(a, i, p, c, colors, mask);
+    for (int b = 0; b < C::BLOCKS; ++b) scales[(long long)i * a.nb + b] = (uint8_t)(c.bytes >> (8 * b));
+    write_colors<DEG, true, NT_COLOR>(a, i, p, c, colors, mask);
 }
 
 // One thread per Gaussian, all views; the features' gradient rows leave through LDS.  Which
@@ -584,6 +629,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, con
     const v3a p = load3(a.xyz + 3LL * i);
     Coef<DEG> c;
     c.load(i, a);
+    c.fold();
     float acc[3 * NF];
 #pragma unroll
     for (int k = 0; k < 3 * NF; ++k) acc[k] = 0.0f;
@@ -613,6 +659,8 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, con
             az = mad(r, mad(-along, z, gz), az);
         }
     }
+#pragma unroll
+    for (int k = 0; k < 3 * NF; ++k) acc[k] *= (float)SH_C[k / 3];
     if (first + lane < a.P) {
         if (dxyz) store3(dxyz + 3LL * i, ax, ay, az);
         if (ddc) store3(ddc + 3LL * i, acc[0], acc[1], acc[2]);
@@ -1102,9 +1150,12 @@ GSR_API int gsr_sh_colors(int P, int V, int degree, int M, const float* xyz, con
     const ShArgs a = sh_args(P, V, M, xyz, dc, dc_stride, codes, scales, campos);
     const unsigned grid = grid_for(P, 1LL << 31);
     hipStream_t st = (hipStream_t)stream;
-#define GSR_SH_COLORS(D)                                                                  \
-    if (mask) k_sh_colors<D, true><<<grid, CP_THREADS, 0, st>>>(a, colors, mask);         \
-    else k_sh_colors<D, false><<<grid, CP_THREADS, 0, st>>>(a, colors, nullptr)
+    const bool past = 12LL * P * V > NT_COLOR_BYTES;
+#define GSR_SH_COLORS(D)                                                                       \
+    if (mask && past) k_sh_colors<D, true, true><<<grid, CP_THREADS, 0, st>>>(a, colors, mask); \
+    else if (mask) k_sh_colors<D, true, false><<<grid, CP_THREADS, 0, st>>>(a, colors, mask);   \
+    else if (past) k_sh_colors<D, false, true><<<grid, CP_THREADS, 0, st>>>(a, colors, nullptr); \
+    else k_sh_colors<D, false, false><<<grid, CP_THREADS, 0, st>>>(a, colors, nullptr)
     if (degree == 0) { GSR_SH_COLORS(0); }
     else if (degree == 1) { GSR_SH_COLORS(1); }
     else if (degree == 2) { GSR_SH_COLORS(2); }
@@ -1123,14 +1174,20 @@ GSR_API int gsr_sh_colors_quantize(int P, int V, int degree, int M, const float*
     const unsigned grid = grid_for(P, 1LL << 31);
     hipStream_t st = (hipStream_t)stream;
     const bool nt = 12LL * M * P > NT_LOAD_BYTES;
-#define GSR_SH_QUANTIZE(D)                                                                                    \
-    if (nt) k_sh_colors_quantize<D, true><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors); \
-    else k_sh_colors_quantize<D, false><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors)
+    const bool past = 12LL * P * V > NT_COLOR_BYTES;
+#define GSR_SH_QUANTIZE_AS(...) \
+    k_sh_colors_quantize<__VA_ARGS__><<<grid, CP_THREADS, 0, st>>>(a, features, codes, scales, mask, colors)
+#define GSR_SH_QUANTIZE(D)                            \
+    if (nt && past) GSR_SH_QUANTIZE_AS(D, true, true); \
+    else if (nt) GSR_SH_QUANTIZE_AS(D, true, false);   \
+    else if (past) GSR_SH_QUANTIZE_AS(D, false, true); \
+    else GSR_SH_QUANTIZE_AS(D, false, false)
     if (degree == 0) { GSR_SH_QUANTIZE(0); }
     else if (degree == 1) { GSR_SH_QUANTIZE(1); }
     else if (degree == 2) { GSR_SH_QUANTIZE(2); }
     else { GSR_SH_QUANTIZE(3); }
 #undef GSR_SH_QUANTIZE
+#undef GSR_SH_QUANTIZE_AS
     return launched("sh_colors_quantize");
 }
 

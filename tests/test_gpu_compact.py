@@ -643,6 +643,39 @@ def test_step_after_eviction():
         assert torch.equal(a._spec.block(a._arena.data, name), b._spec.block(b._arena.data, name)[ids.long()]), name
 
 
+@pytest.mark.parametrize("M,degree", [(16, 3), (16, 0), (9, 2), (4, 1)])
+def test_colors_of_large_calls_equal_those_of_parts(M, degree):
+    """120k Gaussians, 16 views: 23 MB of colours (and 23 of gradients of the features at M = 16), whose rows and colours
+    go past the caches; the parts of 7.7 MB go through them."""
+    import gsr_train as G
+    P, V = 120_001, 16
+    xyz, f, cam, up = (t.to(DEV) for t in scene(P, M, V, 77))
+    q = G.mx4_quantize(f.flatten(1)[:, 3:])
+    dc = f[:, 0].contiguous()
+    leaves = [t.clone().requires_grad_() for t in (xyz, f, dc)]
+    shown = G.sh_colors(xyz, dc, q, cam, degree)
+    held = G.sh_colors(leaves[0], leaves[2], q, cam, degree)
+    trained = G.sh_colors_quantized(leaves[0], leaves[1], cam, degree)
+    gd = torch.autograd.grad(held, (leaves[0], leaves[2]), up)
+    gt = torch.autograd.grad(trained, leaves[:2], up)
+    assert torch.equal(shown, held) and torch.equal(shown, trained)
+    for a in range(0, P, 40_000):
+        part = slice(a, min(P, a + 40_000))
+        x, g = xyz[part].clone().requires_grad_(), f[part].clone().requires_grad_()
+        rows = G.MX4Rows(q.codes[part].contiguous(), q.scales[part].contiguous(), q.width)
+        d = dc[part].clone().requires_grad_()
+        u = up[:, part].contiguous()
+        assert torch.equal(shown[:, part], G.sh_colors(x.detach(), d.detach(), rows, cam, degree))
+        c = G.sh_colors(x, d, rows, cam, degree)
+        assert torch.equal(shown[:, part], c)
+        for have, want in zip(gd, torch.autograd.grad(c, (x, d), u)):
+            assert torch.equal(have[part], want)
+        c = G.sh_colors_quantized(x, g, cam, degree)
+        assert torch.equal(shown[:, part], c)
+        for have, want in zip(gt, torch.autograd.grad(c, (x, g), u)):
+            assert torch.equal(have[part], want)
+
+
 # ---- offsets past 32 bits --------------------------------------------------------------------------
 def test_offsets_past_32_bits():
     """45M Gaussians at degree 3: 2.16e9 feature values, 8.6 GB.  All zero but for the last rows and a few
