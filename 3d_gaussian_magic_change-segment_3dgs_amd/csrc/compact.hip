@@ -759,12 +759,12 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive, DPP r
     return x;
 }
 
-// Exclusive scan over the block's threads; every thread calls it.
+// Exclusive scan over the block's threads; every thread calls it, each time with an s_wave that no
+// thread still reads.
 template <int THREADS>
 __device__ __forceinline__ uint32_t block_scan_excl(uint32_t x, uint32_t* s_wave) {
     const uint32_t inc = wave_scan(x);
     const int wave = threadIdx.x >> 6;
-    __syncthreads();
     if ((threadIdx.x & 63) == 63) s_wave[wave] = inc;
     __syncthreads();
     uint32_t base = 0;
@@ -827,9 +827,6 @@ __device__ __forceinline__ bool keep_digit(uint32_t key, uint32_t prefix, uint32
 template <int PASS>
 __device__ __forceinline__ KeepSel keep_small_pass(const uint32_t (&key)[16], int n, KeepSel st, uint32_t* h,
                                                    uint32_t* s_wave, KeepSel* s_out) {
-    __syncthreads();
-    for (int k = threadIdx.x; k < KEEP_BINS; k += KEEP_SMALL_THREADS) h[k] = 0u;
-    __syncthreads();
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
         uint32_t d;
@@ -843,22 +840,25 @@ __device__ __forceinline__ KeepSel keep_small_pass(const uint32_t (&key)[16], in
 
 __global__ void __launch_bounds__(KEEP_SMALL_THREADS) k_keep_small(KeepArgs a, const float* __restrict__ w,
                                                                    int* __restrict__ ids) {
-    __shared__ uint32_t h[KEEP_BINS];
-    __shared__ uint32_t s_wave[KEEP_SMALL_THREADS / 64];
-    __shared__ KeepSel s_out;
+    // a part for each pass: no barrier between one pass's last reads and the next one's first writes
+    __shared__ uint32_t h[3][KEEP_BINS];
+    __shared__ uint32_t s_wave[4][KEEP_SMALL_THREADS / 64];
+    __shared__ KeepSel s_out[3];
     const KeepGroup G = a.g[blockIdx.x];
     const int n = G.old_end - G.begin, first = threadIdx.x * 16;
     if (G.pick > 0) {  // the whole block
         uint32_t key[16];
         keep_load16(w, (long long)G.begin + first, G.old_end, key);
+        for (int k = threadIdx.x; k < 3 * KEEP_BINS; k += KEEP_SMALL_THREADS) h[0][k] = 0u;
+        __syncthreads();
         KeepSel st = {0u, (uint32_t)G.pick, 0u};
-        st = keep_small_pass<0>(key, n, st, h, s_wave, &s_out);
-        st = keep_small_pass<1>(key, n, st, h, s_wave, &s_out);
+        st = keep_small_pass<0>(key, n, st, h[0], s_wave[0], &s_out[0]);
+        st = keep_small_pass<1>(key, n, st, h[1], s_wave[1], &s_out[1]);
         if (st.count == st.need && st.prefix > 0) {  // all that share 22 bits stay: T just below them, no ties
             st.prefix = (st.prefix << 10) - 1;
             st.need = 0;
         } else {
-            st = keep_small_pass<2>(key, n, st, h, s_wave, &s_out);
+            st = keep_small_pass<2>(key, n, st, h[2], s_wave[2], &s_out[2]);
         }
         uint32_t gt = 0, eq = 0;
 #pragma unroll
@@ -866,7 +866,7 @@ __global__ void __launch_bounds__(KEEP_SMALL_THREADS) k_keep_small(KeepArgs a, c
             gt += first + k < n && key[k] > st.prefix;
             eq += first + k < n && key[k] == st.prefix;
         }
-        const uint32_t before = block_scan_excl<KEEP_SMALL_THREADS>(gt | eq << 16, s_wave);  // at most 16384 each
+        const uint32_t before = block_scan_excl<KEEP_SMALL_THREADS>(gt | eq << 16, s_wave[3]);  // at most 16384 each
         gt = before & 0xFFFFu;
         eq = before >> 16;
 #pragma unroll
@@ -928,7 +928,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_hist(KeepArgs a, KeepWs ws,
 
 // Rows above / equal to T in each tile.
 __global__ void __launch_bounds__(CP_THREADS) k_keep_count(KeepArgs a, KeepWs ws, const float* __restrict__ w) {
-    __shared__ uint32_t s_wave[CP_THREADS / 64];
+    __shared__ uint32_t s_wave[2][CP_THREADS / 64];
     __shared__ KeepSel s_out;
     const int tile = blockIdx.x, g = keep_group_of(a, tile);
     const KeepGroup G = a.g[g];
@@ -937,7 +937,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_count(KeepArgs a, KeepWs ws
         uint32_t key[16];
         const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE + threadIdx.x * 16;
         keep_load16(w, base, G.old_end, key);
-        const uint32_t T = keep_state<3>(a, ws, g, tile, s_wave, &s_out).prefix;
+        const uint32_t T = keep_state<3>(a, ws, g, tile, s_wave[0], &s_out).prefix;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
             gt += base + k < G.old_end && key[k] > T;
@@ -945,7 +945,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_count(KeepArgs a, KeepWs ws
         }
     }
     const uint32_t both = gt | eq << 16;  // at most KEEP_TILE = 4096 of each
-    const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave);
+    const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave[1]);
     if (threadIdx.x == CP_THREADS - 1) ws.count[tile] = make_uint2((before + both) & 0xFFFFu, (before + both) >> 16);
 }
 
@@ -982,7 +982,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
 #pragma unroll
         for (int k = 0; k < 16; ++k)
             if (first + k < G.old_end) both += key[k] > st.prefix ? 1u : key[k] == st.prefix ? 1u << 16 : 0u;
-        const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave);  // (its barriers also end the sum)
+        const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave);  // (its barrier also ends the sum)
         const uint32_t gt0 = s_gt, eq0 = s_eq;
         const uint32_t ties = eq0 < st.need ? st.need - eq0 : 0u;  // left for this tile
         uint32_t gt = before & 0xFFFFu, eq = before >> 16;
@@ -1226,8 +1226,9 @@ GSR_API int gsr_accumulate_weights(int P, const float* weights, long long stride
 }
 
 GSR_API size_t gsr_keep_ws_bytes(int P) {
+    if (P <= KEEP_SMALL) return 0;  // no group is larger
     return keep_hist_bytes() + align_up(GSR_KEEP_MAX_GROUPS * 3 * sizeof(KeepSel)) +
-           align_up(keep_tiles(P > 0 ? (size_t)P : 0) * sizeof(uint2));
+           align_up(keep_tiles((size_t)P) * sizeof(uint2));
 }
 
 GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const gsr_keep_group* groups, int* ids,
@@ -1252,7 +1253,7 @@ GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const g
         most = std::max(most, q.end - q.begin);
     }
     if (a.n == 0) return 0;
-    if (!weights || !ids || !ws) return set_error("[gsr] gsr_keep_heaviest: null buffer");
+    if (!weights || !ids || (!ws && P > KEEP_SMALL)) return set_error("[gsr] gsr_keep_heaviest: null buffer");
     hipStream_t st = (hipStream_t)stream;
     if (most <= KEEP_SMALL) {
         k_keep_small<<<a.n, KEEP_SMALL_THREADS, 0, st>>>(a, weights, ids);

@@ -100,9 +100,11 @@ at::Tensor colors_of(const at::Tensor& xyz, const at::Tensor& dc, const at::Tens
     return colors;
 }
 
+// scales and mask: defined, or behind the codes in one buffer (quantized_of).
 void keep(AutogradContext* ctx, const at::Tensor& xyz, const at::Tensor& campos, const at::Tensor& codes,
           const at::Tensor& scales, const at::Tensor& mask, int64_t degree, int64_t M) {
-    ctx->save_for_backward({xyz, campos, codes, scales, mask});
+    if (scales.defined()) ctx->save_for_backward({xyz, campos, codes, scales, mask});
+    else ctx->save_for_backward({xyz, campos, codes});
     ctx->saved_data["degree"] = degree;
     ctx->saved_data["M"] = M;
 }
@@ -110,8 +112,11 @@ void keep(AutogradContext* ctx, const at::Tensor& xyz, const at::Tensor& campos,
 // The gradients wanted of (dxyz, ddc or dfeatures); a second derivative is refused when it is taken.
 variable_list gradients(AutogradContext* ctx, const at::Tensor& g_in, bool features) {
     const auto sv = ctx->get_saved_variables();
-    const at::Tensor &xyz = sv[0], &campos = sv[1], &codes = sv[2], &scales = sv[3], &mask = sv[4];
+    const at::Tensor &xyz = sv[0], &campos = sv[1], &codes = sv[2];
     const int64_t P = xyz.size(0), M = ctx->saved_data["M"].toInt(), degree = ctx->saved_data["degree"].toInt();
+    const bool apart = sv.size() > 3;
+    const uint8_t* scales = apart ? sv[3].data_ptr<uint8_t>() : codes.data_ptr<uint8_t>() + P * 4 * words(3 * (M - 1));
+    const uint8_t* mask = apart ? sv[4].data_ptr<uint8_t>() : scales + P * blocks(3 * (M - 1));
     Guard guard(xyz.device());
     const bool twice = at::GradMode::is_enabled() && g_in.requires_grad();
     variable_list out(2);
@@ -124,8 +129,7 @@ variable_list gradients(AutogradContext* ctx, const at::Tensor& g_in, bool featu
         float* second = out[1].defined() ? out[1].data_ptr<float>() : nullptr;
         if (P)
             check(gsr_sh_colors_backward((int)P, (int)campos.size(0), (int)degree, (int)M, xyz.data_ptr<float>(),
-                                         code_ptr(codes), scales.data_ptr<uint8_t>(), campos.data_ptr<float>(),
-                                         mask.data_ptr<uint8_t>(), g.data_ptr<float>(),
+                                         code_ptr(codes), scales, campos.data_ptr<float>(), mask, g.data_ptr<float>(),
                                          out[0].defined() ? out[0].data_ptr<float>() : nullptr,
                                          features ? nullptr : second, features ? second : nullptr, cur_stream()));
     }
@@ -157,27 +161,29 @@ struct ShColorsFn : public torch::autograd::Function<ShColorsFn> {
     }
 };
 
+// What the backward needs of a call goes into one buffer: the codes, the scales, the mask.
 at::Tensor quantized_of(const at::Tensor& xyz, const at::Tensor& features, const at::Tensor& campos, int64_t degree,
-                        bool single, at::Tensor& codes, at::Tensor& scales, at::Tensor& mask) {
+                        bool single, at::Tensor& held) {
     const int64_t P = xyz.size(0), V = campos.size(0), M = features.size(1), K = 3 * (M - 1);
-    codes = at::empty({P, 4 * words(K)}, like(xyz, at::kByte));
-    scales = at::empty({P, blocks(K)}, like(xyz, at::kByte));
-    mask = at::empty({V, P}, like(xyz, at::kByte));
+    held = at::empty({P * (4 * words(K) + blocks(K) + V)}, like(xyz, at::kByte));
     at::Tensor colors = colors_for(xyz, V, single);
-    if (P)
+    if (P) {
+        uint8_t* codes = held.data_ptr<uint8_t>();
+        uint8_t* scales = codes + P * 4 * words(K);
         check(gsr_sh_colors_quantize((int)P, (int)V, (int)degree, (int)M, xyz.data_ptr<float>(),
-                                     features.data_ptr<float>(), campos.data_ptr<float>(), code_out(codes),
-                                     scales.data_ptr<uint8_t>(), mask.data_ptr<uint8_t>(), colors.data_ptr<float>(),
-                                     cur_stream()));
+                                     features.data_ptr<float>(), campos.data_ptr<float>(),
+                                     reinterpret_cast<uint32_t*>(codes), scales, scales + P * blocks(K),
+                                     colors.data_ptr<float>(), cur_stream()));
+    }
     return colors;
 }
 
 struct ShColorsQuantizedFn : public torch::autograd::Function<ShColorsQuantizedFn> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& xyz, const at::Tensor& features,
                               const at::Tensor& campos, int64_t degree, bool single) {
-        at::Tensor codes, scales, mask;
-        at::Tensor colors = quantized_of(xyz, features, campos, degree, single, codes, scales, mask);
-        keep(ctx, xyz, campos, codes, scales, mask, degree, features.size(1));
+        at::Tensor held;
+        at::Tensor colors = quantized_of(xyz, features, campos, degree, single, held);
+        keep(ctx, xyz, campos, held, {}, {}, degree, features.size(1));
         return colors;
     }
     static variable_list backward(AutogradContext* ctx, variable_list go) {
@@ -255,8 +261,8 @@ at::Tensor sh_colors_quantized(const at::Tensor& xyz_, const at::Tensor& feature
     const bool single = campos_.dim() == 1;
     const at::Tensor xyz = xyz_.contiguous(), features = features_.contiguous(), campos = views_of(campos_);
     if (wanted(xyz, features)) return ShColorsQuantizedFn::apply(xyz, features, campos, degree, single);
-    at::Tensor codes, scales, mask;
-    return quantized_of(xyz, features, campos, degree, single, codes, scales, mask);
+    at::Tensor held;
+    return quantized_of(xyz, features, campos, degree, single, held);
 }
 
 at::Tensor keep_heaviest(const at::Tensor& weights, const std::vector<std::tuple<int, int, int, int>>& plan) {
@@ -270,9 +276,10 @@ at::Tensor keep_heaviest(const at::Tensor& weights, const std::vector<std::tuple
     at::Tensor ids = at::empty({n}, like(weights, at::kInt));
     if (n) {
         const int P = (int)weights.numel();
-        at::Tensor ws = at::empty({(int64_t)gsr_keep_ws_bytes(P)}, like(weights, at::kByte));
+        const int64_t bytes = (int64_t)gsr_keep_ws_bytes(P);
+        at::Tensor ws = bytes ? at::empty({bytes}, like(weights, at::kByte)) : at::Tensor();
         check(gsr_keep_heaviest(P, weights.data_ptr<float>(), (int)g.size(), g.data(), ids.data_ptr<int>(),
-                                ws.data_ptr(), cur_stream()));
+                                bytes ? ws.data_ptr() : nullptr, cur_stream()));
     }
     return ids;
 }

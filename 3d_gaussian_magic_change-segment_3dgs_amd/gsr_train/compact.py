@@ -378,10 +378,12 @@ def _take(ids, tensors, out, pad):
     K = ids.shape[0]
     if out is not None and len(out) != len(tensors):
         raise RuntimeError("take_rows: one output for each tensor")
-    if _HOST is not None and ids.device.type == "cuda" and \
-            all(isinstance(t, torch.Tensor) for t in tensors + (out or [])):
-        got = _HOST.take_rows(ids, tensors, out or [], pad or [], out is not None)
-        return got if out is None else out
+    if _HOST is not None and ids.device.type == "cuda":
+        try:
+            got = _HOST.take_rows(ids, tensors, out or [], pad or [], out is not None)
+            return got if out is None else out
+        except TypeError:  # something that is no tensor: refused below
+            pass
     if out is None:
         out = [torch.empty((K,) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device) if isinstance(t, torch.Tensor)
                else None for t in tensors]

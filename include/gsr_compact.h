@@ -72,7 +72,8 @@ GSR_API int gsr_accumulate_weights(int P, const float* weights, long long stride
  * rows and, of the others, the heaviest by weight (ties: the lowest row; NaN below
  * everything, -0 = +0).  ids gets the kept rows in ascending order, group after group
  * (sum of keep entries).  Groups are ascending and do not overlap; rows in no group are
- * not kept.  ws: gsr_keep_ws_bytes(P) bytes, 16-B aligned, used by this call only. */
+ * not kept.  ws: gsr_keep_ws_bytes(P) bytes (0 for small P: then ws may be NULL), 16-B aligned,
+ * used by this call only. */
 #define GSR_KEEP_MAX_GROUPS 64
 typedef struct gsr_keep_group {
     int begin, end;
