@@ -696,9 +696,11 @@ __global__ void __launch_bounds__(CP_THREADS) k_accumulate_weights(int P, const 
 // lowest first); then the ids are written in order.  Every count is an integer, so the result
 // does not depend on the order of the atomics.
 //   One block per group does it all for groups of up to KEEP_SMALL rows, the keys in registers;
-// larger groups take a launch per pass over tiles of KEEP_TILE rows: what is read, 4 bytes a row
-// and pass from the caches, is less than what the launches and their dependences cost.
-constexpr int KEEP_TILE = CP_THREADS * 16;  // rows per block
+// larger groups take a launch per pass, the last of which also counts for each tile what the kernel
+// that writes the ids needs: what is read, 4 bytes a row and pass from the caches, is less than what
+// the launches and their dependences cost (five launches; 1M rows 26 us, with a sixth for the counts 29).
+// Weights that are all equal queue at one counter: 1M rows 33 us.
+constexpr int KEEP_TILE = CP_THREADS * 16;  // rows a block holds at once
 constexpr int KEEP_BINS = 2048;
 constexpr int KEEP_SMALL_THREADS = 1024, KEEP_SMALL = KEEP_SMALL_THREADS * 16;
 
@@ -709,7 +711,7 @@ struct KeepGroup {
     int tile0;  // first tile
 };
 struct KeepArgs {
-    int n, tiles;
+    int n, tiles, rounds;
     KeepGroup g[GSR_KEEP_MAX_GROUPS];
 };
 struct KeepSel {
@@ -719,16 +721,29 @@ struct KeepSel {
 struct KeepWs {
     uint32_t* hist;  // [groups][3][KEEP_BINS]
     KeepSel* sel;    // [groups][3]
-    uint2* count;    // [tiles] rows above T, rows equal to T
+    uint32_t* above; // [tiles] rows above the first 22 bits of T (with those that share them, if all of them stay)
+    uint16_t* from;  // [tiles][KEEP_LOW] rows that share them with low bits of at least the index
 };
-inline size_t keep_tiles(size_t P) { return P / KEEP_TILE + GSR_KEEP_MAX_GROUPS + 1; }
+constexpr int KEEP_LOW = 1024;  // the last pass's bins
+// A block takes so many times KEEP_TILE rows of a group (a tile) that there are about 1024 tiles: fewer
+// histograms to add up, and what the last kernel reads of the tiles before its own grows with their
+// square (10M rows, one piece a tile and three: 130 -> 80 us; 45M, one and eleven: 702 -> 183; 3M, one and
+// two: 47 -> 41 with the weights in the caches, but an eviction with its rows 181 -> 184, so one).
+// At most 15: a tile's counts are kept in 16 bits.
+inline int keep_rounds(size_t P) {
+    const size_t r = (P / KEEP_TILE + 1023) / 1024;
+    return (int)(r < 1 ? 1 : r > 15 ? 15 : r);
+}
+inline size_t keep_tiles(size_t P) { return P / ((size_t)KEEP_TILE * keep_rounds(P)) + GSR_KEEP_MAX_GROUPS + 1; }
 inline size_t keep_hist_bytes() { return (size_t)GSR_KEEP_MAX_GROUPS * 3 * KEEP_BINS * 4; }
-inline KeepWs keep_ws(void* p) {
+inline KeepWs keep_ws(void* p, size_t tiles) {
     char* c = static_cast<char*>(p);
     KeepWs w;
     w.hist = reinterpret_cast<uint32_t*>(c);
     w.sel = reinterpret_cast<KeepSel*>(c + keep_hist_bytes());
-    w.count = reinterpret_cast<uint2*>(c + keep_hist_bytes() + align_up(GSR_KEEP_MAX_GROUPS * 3 * sizeof(KeepSel)));
+    c += keep_hist_bytes() + align_up(GSR_KEEP_MAX_GROUPS * 3 * sizeof(KeepSel));
+    w.above = reinterpret_cast<uint32_t*>(c);
+    w.from = reinterpret_cast<uint16_t*>(c + align_up(tiles * sizeof(uint32_t)));
     return w;
 }
 
@@ -823,6 +838,9 @@ __device__ __forceinline__ bool keep_digit(uint32_t key, uint32_t prefix, uint32
     return PASS == 0 || (PASS == 1 ? key >> 21 : key >> 10) == prefix;
 }
 
+// All rows that share the 22 bits found in two passes stay: T is just below them, without ties.
+__device__ __forceinline__ bool keep_early(KeepSel st) { return st.count == st.need && st.prefix > 0; }
+
 // One pass over the keys of a small group: the digits found before it -> one more.
 template <int PASS>
 __device__ __forceinline__ KeepSel keep_small_pass(const uint32_t (&key)[16], int n, KeepSel st, uint32_t* h,
@@ -854,7 +872,7 @@ __global__ void __launch_bounds__(KEEP_SMALL_THREADS) k_keep_small(KeepArgs a, c
         KeepSel st = {0u, (uint32_t)G.pick, 0u};
         st = keep_small_pass<0>(key, n, st, h[0], s_wave[0], &s_out[0]);
         st = keep_small_pass<1>(key, n, st, h[1], s_wave[1], &s_out[1]);
-        if (st.count == st.need && st.prefix > 0) {  // all that share 22 bits stay: T just below them, no ties
+        if (keep_early(st)) {
             st.prefix = (st.prefix << 10) - 1;
             st.need = 0;
         } else {
@@ -896,81 +914,97 @@ __device__ __forceinline__ KeepSel keep_state(const KeepArgs& a, const KeepWs& w
     if (PASS > 1) prev = ws.sel[g * 3 + PASS - 2];
     const KeepSel b = find_bin<CP_THREADS>(ws.hist + ((size_t)g * 3 + PASS - 1) * KEEP_BINS, prev.need, s_wave, s_out);
     const KeepSel now = {(prev.prefix << (PASS == 3 ? 10 : 11)) | b.prefix, b.need, b.count};
-    if (tile == a.g[g].tile0 && threadIdx.x == 0) ws.sel[g * 3 + PASS - 1] = now;
+    if (PASS < 3 && tile == a.g[g].tile0 && threadIdx.x == 0) ws.sel[g * 3 + PASS - 1] = now;
     return now;
 }
 
-template <int PASS>
+// LAST: the rows above the 22 bits are counted for each tile, and those that share them by their low bits
+// (running sums from the top, so that the next kernel reads two numbers a tile whatever T is) -- or
+// with the others, if all of them stay.
+// MANY: more than one piece a tile (the loop costs 1M rows, which are one each, 27.7 us instead of 26.1).
+template <int PASS, bool MANY>
 __global__ void __launch_bounds__(CP_THREADS) k_keep_hist(KeepArgs a, KeepWs ws, const float* __restrict__ w) {
-    __shared__ uint32_t h[KEEP_BINS];
-    __shared__ uint32_t s_wave[CP_THREADS / 64];
+    constexpr bool LAST = PASS == 2;
+    constexpr int BINS = LAST ? KEEP_LOW : KEEP_BINS;
+    __shared__ uint32_t h[BINS];
+    __shared__ uint32_t s_wave[3][CP_THREADS / 64];
     __shared__ KeepSel s_out;
     const int tile = blockIdx.x, g = keep_group_of(a, tile);
     const KeepGroup G = a.g[g];
     if (G.pick == 0) return;  // nothing to look for (the whole block)
     uint32_t key[16];
-    const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE + threadIdx.x * 16;
+    const int rounds = MANY ? a.rounds : 1;
+    long long base = G.begin + (long long)(tile - G.tile0) * rounds * KEEP_TILE + threadIdx.x * 16;
     keep_load16(w, base, G.old_end, key);
-    for (int k = threadIdx.x; k < KEEP_BINS; k += CP_THREADS) h[k] = 0u;
-    const KeepSel st = keep_state<PASS>(a, ws, g, tile, s_wave, &s_out);
+    for (int k = threadIdx.x; k < BINS; k += CP_THREADS) h[k] = 0u;
+    const KeepSel st = keep_state<PASS>(a, ws, g, tile, s_wave[0], &s_out);
     __syncthreads();
+    const bool early = LAST && keep_early(st);
+    uint32_t above = 0;
+    for (int round = 1;; ++round) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        uint32_t d;
-        const bool in = keep_digit<PASS>(key[k], st.prefix, d) && base + k < G.old_end;
-        keep_add(h, d, in);
+        for (int k = 0; k < 16; ++k) {
+            uint32_t d;
+            const bool in = base + k < G.old_end, same = keep_digit<PASS>(key[k], st.prefix, d);
+            if constexpr (LAST) above += in && (key[k] >> 10 > st.prefix || (same && early));
+            keep_add(h, d, in && same && !early);
+        }
+        base += KEEP_TILE;
+        if (!MANY || round == rounds || base - threadIdx.x * 16 >= G.old_end) break;  // the whole block
+        keep_load16(w, base, G.old_end, key);
+    }
+    if constexpr (LAST) {
+        const uint32_t before = block_scan_excl<CP_THREADS>(above, s_wave[1]);
+        if (threadIdx.x == CP_THREADS - 1) ws.above[tile] = before + above;
+        if (early) return;  // the whole block
     }
     __syncthreads();
     uint32_t* out = ws.hist + ((size_t)g * 3 + PASS) * KEEP_BINS;
-    for (int k = threadIdx.x; k < KEEP_BINS; k += CP_THREADS)
+    for (int k = threadIdx.x; k < BINS; k += CP_THREADS)
         if (h[k]) atomicAdd(&out[k], h[k]);
-}
-
-// Rows above / equal to T in each tile.
-__global__ void __launch_bounds__(CP_THREADS) k_keep_count(KeepArgs a, KeepWs ws, const float* __restrict__ w) {
-    __shared__ uint32_t s_wave[2][CP_THREADS / 64];
-    __shared__ KeepSel s_out;
-    const int tile = blockIdx.x, g = keep_group_of(a, tile);
-    const KeepGroup G = a.g[g];
-    uint32_t gt = 0, eq = 0;
-    if (G.pick > 0) {
-        uint32_t key[16];
-        const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE + threadIdx.x * 16;
-        keep_load16(w, base, G.old_end, key);
-        const uint32_t T = keep_state<3>(a, ws, g, tile, s_wave[0], &s_out).prefix;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            gt += base + k < G.old_end && key[k] > T;
-            eq += base + k < G.old_end && key[k] == T;
-        }
+    if constexpr (LAST) {
+        const int first = KEEP_LOW - 4 - 4 * (int)threadIdx.x;  // four bins a thread, from the top
+        const uint32_t h3 = h[first + 3], h2 = h3 + h[first + 2], h1 = h2 + h[first + 1], h0 = h1 + h[first];
+        const uint32_t b = block_scan_excl<CP_THREADS>(h0, s_wave[2]);
+        const uint32_t lo = (b + h0) | (b + h1) << 16, hi = (b + h2) | (b + h3) << 16;
+        *reinterpret_cast<uint2*>(ws.from + (size_t)tile * KEEP_LOW + first) = make_uint2(lo, hi);
     }
-    const uint32_t both = gt | eq << 16;  // at most KEEP_TILE = 4096 of each
-    const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave[1]);
-    if (threadIdx.x == CP_THREADS - 1) ws.count[tile] = make_uint2((before + both) & 0xFFFFu, (before + both) >> 16);
 }
 
 // A tile's kept rows: ranked by a scan over the threads (16 rows each, in order), gathered in LDS
 // and written in one piece behind those of the tiles before.
+template <bool MANY>
 __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws, const float* __restrict__ w,
                                                            int* __restrict__ ids) {
-    __shared__ uint32_t s_wave[CP_THREADS / 64];
+    __shared__ uint32_t s_wave[2][CP_THREADS / 64];
     __shared__ uint32_t s_gt, s_eq;
     __shared__ int s_ids[KEEP_TILE];
     __shared__ uint32_t s_n;
+    __shared__ KeepSel s_out;
     const int tile = blockIdx.x, g = keep_group_of(a, tile);
     const KeepGroup G = a.g[g];
-    const long long base = G.begin + (long long)(tile - G.tile0) * KEEP_TILE, first = base + threadIdx.x * 16;
+    const int rounds = MANY ? a.rounds : 1;
+    const long long span = (long long)rounds * KEEP_TILE, base = G.begin + (tile - G.tile0) * span;
     if (G.pick > 0 && base < G.old_end) {  // the whole block
+        long long first = base + threadIdx.x * 16;
         uint32_t key[16];
         keep_load16(w, first, G.old_end, key);
-        const KeepSel st = ws.sel[g * 3 + 2];
+        KeepSel st = ws.sel[g * 3 + 1];
         if (threadIdx.x == 0) s_gt = s_eq = 0;
-        __syncthreads();
         uint2 sum = {0u, 0u};
-        for (int t = G.tile0 + threadIdx.x; t < tile; t += CP_THREADS) {
-            const uint2 c = ws.count[t];
-            sum.x += c.x;
-            sum.y += c.y;
+        for (int t = G.tile0 + threadIdx.x; t < tile; t += CP_THREADS) sum.x += ws.above[t];
+        if (keep_early(st)) {
+            st = {(st.prefix << 10) - 1, 0u, 0u};
+            __syncthreads();
+        } else {
+            st = keep_state<3>(a, ws, g, tile, s_wave[0], &s_out);  // (its barriers order s_gt and s_eq too)
+            const uint32_t low = st.prefix & (KEEP_LOW - 1);
+            for (int t = G.tile0 + threadIdx.x; t < tile; t += CP_THREADS) {
+                const uint16_t* f = ws.from + (size_t)t * KEEP_LOW + low;
+                const uint32_t up = low + 1 < KEEP_LOW ? f[1] : 0u;
+                sum.x += up;
+                sum.y += f[0] - up;
+            }
         }
         sum.x = wave_scan(sum.x);
         sum.y = wave_scan(sum.y);
@@ -978,29 +1012,43 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
             atomicAdd(&s_gt, sum.x);
             atomicAdd(&s_eq, sum.y);
         }
-        uint32_t both = 0;
+        uint32_t gt0 = 0, eq0 = 0;  // rows above / equal to T before this round's
+        for (int round = 1;; ++round) {
+            uint32_t both = 0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-            if (first + k < G.old_end) both += key[k] > st.prefix ? 1u : key[k] == st.prefix ? 1u << 16 : 0u;
-        const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave);  // (its barrier also ends the sum)
-        const uint32_t gt0 = s_gt, eq0 = s_eq;
-        const uint32_t ties = eq0 < st.need ? st.need - eq0 : 0u;  // left for this tile
-        uint32_t gt = before & 0xFFFFu, eq = before >> 16;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            if (first + k < G.old_end) {
-                const bool up = key[k] > st.prefix, tie = key[k] == st.prefix;
-                if (up || (tie && eq < ties)) s_ids[gt + (eq < ties ? eq : ties)] = (int)(first + k);
-                gt += up;
-                eq += tie;
+            for (int k = 0; k < 16; ++k)
+                if (first + k < G.old_end) both += key[k] > st.prefix ? 1u : key[k] == st.prefix ? 1u << 16 : 0u;
+            const uint32_t before = block_scan_excl<CP_THREADS>(both, s_wave[1]);
+            if (round == 1) {  // (the scan's barrier also ends the sum)
+                gt0 = s_gt;
+                eq0 = s_eq;
             }
+            const uint32_t ties = eq0 < st.need ? st.need - eq0 : 0u;  // left for this round
+            uint32_t gt = before & 0xFFFFu, eq = before >> 16;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                if (first + k < G.old_end) {
+                    const bool up = key[k] > st.prefix, tie = key[k] == st.prefix;
+                    if (up || (tie && eq < ties)) s_ids[gt + (eq < ties ? eq : ties)] = (int)(first + k);
+                    gt += up;
+                    eq += tie;
+                }
+            }
+            if (threadIdx.x == CP_THREADS - 1) s_n = gt | eq << 16;  // at most KEEP_TILE = 4096 of each
+            first += KEEP_TILE;
+            const bool more = MANY && round < rounds && first - threadIdx.x * 16 < G.old_end;  // the whole block
+            if (more) keep_load16(w, first, G.old_end, key);
+            __syncthreads();
+            gt = s_n & 0xFFFFu;
+            eq = s_n >> 16;
+            int* out = ids + G.out + gt0 + (eq0 < st.need ? eq0 : st.need);
+            for (uint32_t k = threadIdx.x; k < gt + (eq < ties ? eq : ties); k += CP_THREADS) out[k] = s_ids[k];
+            if (!more) break;
+            gt0 += gt;  // (the next scan's barrier is behind all reads of s_ids and s_n)
+            eq0 += eq;
         }
-        if (threadIdx.x == CP_THREADS - 1) s_n = gt + (eq < ties ? eq : ties);
-        __syncthreads();
-        int* out = ids + G.out + gt0 + (eq0 < st.need ? eq0 : st.need);
-        for (uint32_t k = threadIdx.x; k < s_n; k += CP_THREADS) out[k] = s_ids[k];
     }
-    const long long lo = base > G.old_end ? base : G.old_end, hi = base + KEEP_TILE < G.end ? base + KEEP_TILE : G.end;
+    const long long lo = base > G.old_end ? base : G.old_end, hi = base + span < G.end ? base + span : G.end;
     for (long long i = lo + threadIdx.x; i < hi; i += CP_THREADS) ids[G.out + G.pick + (i - G.old_end)] = (int)i;
 }
 
@@ -1228,7 +1276,7 @@ GSR_API int gsr_accumulate_weights(int P, const float* weights, long long stride
 GSR_API size_t gsr_keep_ws_bytes(int P) {
     if (P <= KEEP_SMALL) return 0;  // no group is larger
     return keep_hist_bytes() + align_up(GSR_KEEP_MAX_GROUPS * 3 * sizeof(KeepSel)) +
-           align_up(keep_tiles((size_t)P) * sizeof(uint2));
+           align_up(keep_tiles((size_t)P) * sizeof(uint32_t)) + keep_tiles((size_t)P) * KEEP_LOW * sizeof(uint16_t);
 }
 
 GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const gsr_keep_group* groups, int* ids,
@@ -1237,6 +1285,8 @@ GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const g
         return set_error("[gsr] gsr_keep_heaviest: at most " + std::to_string(GSR_KEEP_MAX_GROUPS) + " groups a call");
     if (n_groups > 0 && !groups) return set_error("[gsr] gsr_keep_heaviest: null groups");
     KeepArgs a{};
+    a.rounds = keep_rounds((size_t)P);
+    const long long span = (long long)KEEP_TILE * a.rounds;
     int last = 0, most = 0;
     long long out = 0;
     for (int g = 0; g < n_groups; ++g) {
@@ -1248,7 +1298,7 @@ GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const g
         last = q.end;
         if (q.keep == 0) continue;  // nothing to write
         a.g[a.n++] = {q.begin, q.end, q.end - q.recent, q.keep - q.recent, (int)out, a.tiles};
-        a.tiles += (q.end - q.begin + KEEP_TILE - 1) / KEEP_TILE;
+        a.tiles += (int)((q.end - q.begin + span - 1) / span);
         out += q.keep;
         most = std::max(most, q.end - q.begin);
     }
@@ -1259,14 +1309,17 @@ GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const g
         k_keep_small<<<a.n, KEEP_SMALL_THREADS, 0, st>>>(a, weights, ids);
         return launched("keep_heaviest");
     }
-    const KeepWs w = keep_ws(ws);
+    const KeepWs w = keep_ws(ws, keep_tiles((size_t)P));
     const int words = a.n * 3 * KEEP_BINS;
     k_keep_clear<<<grid_for(words, 1024), CP_THREADS, 0, st>>>(w.hist, words);
-    k_keep_hist<0><<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);
-    k_keep_hist<1><<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);
-    k_keep_hist<2><<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);
-    k_keep_count<<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);
-    k_keep_write<<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights, ids);
+#define GSR_KEEP(MANY)                                                       \
+    k_keep_hist<0, MANY><<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);      \
+    k_keep_hist<1, MANY><<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);      \
+    k_keep_hist<2, MANY><<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights);      \
+    k_keep_write<MANY><<<a.tiles, CP_THREADS, 0, st>>>(a, w, weights, ids)
+    if (a.rounds > 1) { GSR_KEEP(true); }
+    else { GSR_KEEP(false); }
+#undef GSR_KEEP
     return launched("keep_heaviest");
 }
 

@@ -390,6 +390,34 @@ def test_keep_heaviest_groups():
     check_keep(w[:5000].view(5000, 1), 77)  # [P, 1], as the model holds them
 
 
+@pytest.mark.parametrize("kind", ["heavy", "equal", "whole"])
+def test_keep_heaviest_of_many_rows(kind):
+    """9M rows (a block takes two pieces of a tile) and 17M (three): in one group, and in groups of unequal size whose
+    ends lie inside a piece."""
+    g = gen(9)
+    n = 9_000_001 if kind != "whole" else 17_000_003
+    w = torch.exp(torch.randn(n, generator=g) * 2)
+    if kind == "equal":
+        w[:] = 0.5
+    elif kind == "whole":  # few values, most of them often
+        w = (w * 4).floor()
+    import gsr_train as G
+    w = w.to(DEV)
+
+    def want(groups, budget, recent):
+        keep = torch.zeros(n, dtype=torch.bool, device=DEV)
+        for (a, b), r in zip(groups, recent):
+            k = min(budget, b - a)
+            r = min(r, k)
+            keep[a + torch.sort(w[a:b - r], descending=True, stable=True)[1][:k - r]] = True
+            keep[b - r:b] = True
+        return torch.nonzero(keep).flatten().int()
+
+    assert torch.equal(G.keep_heaviest(w, n * 3 // 5), want([(0, n)], n * 3 // 5, [0]))
+    groups, recent = [(0, 5000), (5000, 4_105_001), (4_200_000, 4_208_193), (4_208_193, n)], [0, 100_000, 5, 9]
+    assert torch.equal(G.keep_heaviest(w, n // 3, groups, recent), want(groups, n // 3, recent))
+
+
 def test_keep_heaviest_twice_at_once_and_on_other_streams():
     import gsr_train as G
     w = [torch.exp(torch.randn(200_000, generator=gen(k))).to(DEV) for k in range(4)]
