@@ -1337,7 +1337,7 @@ GSR_API int gsr_take_rows(int K, const int* ids, int n, const gsr_rows* tensors,
     // what is written is neither read nor written by another tensor of the call
     struct Range {
         uintptr_t lo, hi;
-        bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
+        bool meets(const Range& o) const { return lo < hi && o.lo < o.hi && lo < o.hi && o.lo < hi; }
     };
     auto written = [&](const gsr_rows& t) -> Range {
         return {(uintptr_t)t.dst, (uintptr_t)t.dst + 4 * ((uintptr_t)K * t.width + t.pad)};

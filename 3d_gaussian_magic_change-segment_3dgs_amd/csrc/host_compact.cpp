@@ -11,6 +11,7 @@
 #include <stdexcept>
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "gsr_compact.h"
@@ -192,8 +193,37 @@ struct ShColorsQuantizedFn : public torch::autograd::Function<ShColorsQuantizedF
     }
 };
 
-bool wanted(const at::Tensor& a, const at::Tensor& b) {
-    return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad());
+// In a capture, every node that the gradients will flow through has to belong to the capturing stream: the
+// backward pass would make another node's stream wait for it, which breaks the capture beyond repair.  Such
+// nodes are an eager graph's: one that the inputs come from, or the accumulators of the same leaves, which live
+// as long as any graph of them.
+void check_capture(const char* what, const at::Tensor& a, const at::Tensor& b) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const auto here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA();
+    if (hipStreamIsCapturing(here.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+    std::unordered_set<torch::autograd::Node*> seen;
+    for (const at::Tensor* t : {&a, &b}) {
+        if (!t->requires_grad()) continue;
+        auto node = t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (node && seen.insert(node.get()).second) todo.push_back(node);
+    }
+    while (!todo.empty()) {
+        const auto node = todo.back();
+        todo.pop_back();
+        const auto stream = node->stream();
+        if (stream && *stream != here.unwrap())
+            refuse(std::string(what) + ": captured while an eager graph of the same tensors is alive (" + node->name() +
+                   " is on another stream): drop it, or make it in the capture");
+        for (const auto& e : node->next_edges())
+            if (e.function && seen.insert(e.function.get()).second) todo.push_back(e.function);
+    }
+}
+
+bool wanted(const char* what, const at::Tensor& a, const at::Tensor& b) {
+    const bool yes = at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad());
+    if (yes) check_capture(what, a, b);
+    return yes;
 }
 
 }  // namespace
@@ -236,11 +266,11 @@ at::Tensor sh_colors(const at::Tensor& xyz_, const at::Tensor& features_dc, cons
     check_device("sh_colors", "rest", codes, xyz_);
     check_device("sh_colors", "campos", campos_, xyz_);
     Guard guard(xyz_.device());
-    const bool single = campos_.dim() == 1;
+    const bool single = campos_.dim() == 1, grad = wanted("sh_colors", xyz_, features_dc);
     const at::Tensor xyz = xyz_.contiguous(), campos = views_of(campos_);
     at::Tensor dc = dims == 3 ? features_dc.squeeze(1) : features_dc;
     if (P && (dc.stride(1) != 1 || (P > 1 && dc.stride(0) < 3))) dc = dc.contiguous();
-    if (wanted(xyz, dc)) return ShColorsFn::apply(xyz, dc, campos, codes, scales, degree, M, single);
+    if (grad) return ShColorsFn::apply(xyz, dc, campos, codes, scales, degree, M, single);
     return colors_of(xyz, dc, campos, codes, scales, degree, M, single, nullptr);
 }
 
@@ -258,9 +288,9 @@ at::Tensor sh_colors_quantized(const at::Tensor& xyz_, const at::Tensor& feature
     check_device(what, "features", features_, xyz_);
     check_device(what, "campos", campos_, xyz_);
     Guard guard(xyz_.device());
-    const bool single = campos_.dim() == 1;
+    const bool single = campos_.dim() == 1, grad = wanted(what, xyz_, features_);
     const at::Tensor xyz = xyz_.contiguous(), features = features_.contiguous(), campos = views_of(campos_);
-    if (wanted(xyz, features)) return ShColorsQuantizedFn::apply(xyz, features, campos, degree, single);
+    if (grad) return ShColorsQuantizedFn::apply(xyz, features, campos, degree, single);
     at::Tensor held;
     return quantized_of(xyz, features, campos, degree, single, held);
 }

@@ -88,6 +88,14 @@ def reduce_densification_stats(xyz_gradient_accum, denom, max_radii2D, group=Non
     dist.all_reduce(max_radii2D, op=dist.ReduceOp.MAX, group=group)
 
 
+def reduce_contribution(contribution, group=None):
+    """Sum the blend weights that the ranks accumulated over their own views, in place, before
+    GaussianModel.evict: every rank then keeps the same Gaussians.  (Sums of sums: clear
+    `contribution` before the next views are added.)"""
+    native_fence()
+    dist.all_reduce(contribution, op=dist.ReduceOp.SUM, group=group)
+
+
 def exchange_bytes(world, views_per_rank, M=16):
     """Bytes per Gaussian that each rank sends (ring model) for both exchanges."""
     n, b = int(world), int(views_per_rank)

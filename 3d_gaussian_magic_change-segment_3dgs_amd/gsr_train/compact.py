@@ -15,7 +15,9 @@ csrc/compact.hip).
 
 All tensors are float32 (ids int32, codes and scales uint8) on one GPU; a call uses that
 GPU's current stream, takes its workspace from torch's allocator and never waits for the
-device, so it can be captured into a graph."""
+device, so it can be captured into a graph.  A pass with gradients is captured forward and
+backward together, with no eager graph of the same leaves alive: that is refused, since the
+captured backward pass would have to wait on the eager graph's stream."""
 import ctypes
 
 import torch
@@ -170,6 +172,13 @@ def _sh_check(what, xyz, campos, degree, M):
                            f"(degree {degree}, {M} coefficients)")
 
 
+def _capture_check(what, *tensors):
+    """The compiled binding looks for eager graphs of the same tensors, whose streams a captured backward pass
+    must not touch; here there is no way to."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors) and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: capturing a pass with gradients needs the compiled host binding (gsr_host)")
+
+
 def _buffers(xyz, V, single, grad):
     """(colors [V, P, 3] or [P, 3], mask [V, P] for the backward or None)."""
     P, dev = xyz.shape[0], xyz.device
@@ -275,6 +284,7 @@ def sh_colors(xyz, features_dc, rest, campos, degree):
     if rest.rows != P:
         raise RuntimeError(f"sh_colors: rest must have {P} rows (got {rest.rows})")
     _on_gpu("sh_colors", xyz, features_dc=features_dc, rest=rest, campos=campos)
+    _capture_check("sh_colors", xyz, features_dc)
     dc = features_dc.reshape(P, 3)
     if P and (dc.stride(1) != 1 or (P > 1 and dc.stride(0) < 3)):
         dc = dc.contiguous()
@@ -297,6 +307,7 @@ def sh_colors_quantized(xyz, features, campos, degree):
     if features.shape[0] != xyz.shape[0]:
         raise RuntimeError(f"{what}: features must have {xyz.shape[0]} rows (got {features.shape[0]})")
     _on_gpu(what, xyz, features=features, campos=campos)
+    _capture_check(what, xyz, features)
     return _ShColorsQuantized.apply(xyz.contiguous(), features.contiguous(),
                                     campos.detach().reshape(-1, 3).contiguous(), int(degree), campos.dim() == 1)
 
@@ -371,6 +382,8 @@ def take_rows(ids, tensors, out=None):
     _typed("take_rows", torch.int32, ids=ids)
     if ids.dim() != 1 or not ids.is_contiguous():
         raise RuntimeError("take_rows: ids must be contiguous, of shape (K,)")
+    if ids.shape[0] >= 2 ** 31:
+        raise RuntimeError("take_rows: at most 2^31 - 1 ids")
     return _take(ids, list(tensors), None if out is None else list(out), None)
 
 

@@ -192,3 +192,42 @@ def test_oracle_basis_is_orthonormal(degree):
     b = O.sh_values(d, degree)
     # the constants are written with 16 digits or less: 1e-12
     assert torch.allclose((b * w[:, None]).T @ b, torch.eye(b.shape[1], dtype=torch.float64), atol=1e-12)
+
+
+def test_take_rows_of_nothing_overlaps_nothing():
+    """An empty destination or source inside another tensor's range is no clash."""
+    from gsr_train import compact as T
+    table = (T._Rows * 2)((4096, 4160, 4, 0, 0), (4096, 4104, 0, 64, 0))
+    assert T._lib.gsr_take_rows(0, 64, 2, table, None) == 0
+    table = (T._Rows * 1)((4100, 4096, 2, 0, 0))
+    assert T._lib.gsr_take_rows(0, 64, 1, table, None) == 0
+
+
+def _contribution_worker(rank, world, port, out_q):
+    import sys
+    sys.path[:0] = [ROOT, os.path.join(ROOT, "3d_gaussian_magic_change-segment_3dgs_amd")]
+    import torch.distributed as dist
+    from gsr_tools import dp
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=world)
+    weights = torch.rand(100, 1, generator=torch.Generator().manual_seed(rank))
+    dp.reduce_contribution(weights)
+    out_q.put((rank, weights.numpy().copy()))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_contribution_reduction_gloo_ws2():
+    """Every rank gets the same sums, bit for bit: what evict() keeps is the same everywhere."""
+    import torch.multiprocessing as mp
+    from test_dist_cpu import _free_port
+    ctx = mp.get_context("spawn")
+    q, port = ctx.Queue(), _free_port()
+    procs = [ctx.Process(target=_contribution_worker, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    res = dict(q.get(timeout=120) for _ in range(2))
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    a, b = (torch.rand(100, 1, generator=torch.Generator().manual_seed(r)).numpy() for r in range(2))
+    assert np.array_equal(res[0], a + b) and np.array_equal(res[1], res[0])

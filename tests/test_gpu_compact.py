@@ -465,6 +465,12 @@ def test_take_rows_refuses_an_output_that_overlaps(monkeypatch):
             G.take_rows(ids, [x, x.clone()], out=[torch.empty_like(x), x])
 
 
+def test_take_rows_refuses_more_ids_than_an_int_counts():
+    import gsr_train as G
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        G.take_rows(torch.empty(2 ** 31, dtype=torch.int32, device=DEV), [torch.zeros(3, 0, device=DEV)])
+
+
 def test_take_rows_of_ids_outside():
     import gsr_train as G
     x = torch.randn(10, 3, device=DEV)
@@ -803,3 +809,52 @@ def test_two_graphs_do_not_share_a_workspace():
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("through_a_view", [False, True])
+def test_capture_is_refused_while_an_eager_graph_of_the_leaves_lives(through_a_view):
+    """The accumulator of a leaf keeps the stream it was made on for as long as a graph of the leaf lives; a captured
+    backward pass must not reach it.  Without that graph the capture works."""
+    import gsr_train as G
+    xyz, f, cam, up = scene(300, 4, 1, 5)
+    x, fg = xyz.to(DEV).requires_grad_(), f.to(DEV).requires_grad_()
+    cam, up = cam.to(DEV), up.to(DEV)
+    q = G.mx4_quantize(fg.detach().flatten(1)[:, 3:])
+
+    def trained():
+        return G.sh_colors_quantized(x[:] if through_a_view else x, fg, cam, 1)
+
+    def shown():
+        return G.sh_colors(x[:] if through_a_view else x, fg.detach()[:, 0], q, cam, 1)
+
+    for call in (trained, shown):
+        eager = call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph of the same tensors"):
+            with torch.cuda.graph(graph):
+                call()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):  # without gradients nothing is in the way
+            with torch.no_grad():
+                call()
+        (want,) = torch.autograd.grad(eager, (x,), up)
+        del eager
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            (got,) = torch.autograd.grad(call(), (x,), up)
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+
+def test_capture_with_gradients_needs_the_compiled_binding(monkeypatch):
+    import gsr_train as G
+    from gsr_train import compact as T
+    xyz, f, cam, _ = scene(40, 4, 1, 6)
+    x, fg, cam = xyz.to(DEV).requires_grad_(), f.to(DEV), cam.to(DEV)
+    monkeypatch.setattr(T, "_HOST", None)
+    with pytest.raises(RuntimeError, match="gsr_host"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            G.sh_colors_quantized(x, fg, cam, 1)
