@@ -111,7 +111,8 @@ __device__ __forceinline__ uint32_t max_bits(uint32_t m, v4a v) {
 }
 
 // Four lanes per block, eight values (one code word) each; the four share the largest |x| through
-// DPP.  A thread takes MXQ_PER such pieces, their loads in flight together.
+// DPP.  A thread takes MXQ_PER such pieces, their loads in flight together.  Bound by memory: 1M rows of 45
+// (206 MB, with the 12 bytes between them 218) 35 us, 6.2 TB/s.
 constexpr int MXQ_PER = 2, MXQ_SPAN = CP_THREADS / 4 * MXQ_PER;
 __global__ void __launch_bounds__(CP_THREADS) k_mx4_quantize(long long R, int K, Tiling t, const float* __restrict__ x,
                                                              long long stride, uint32_t* __restrict__ codes,
@@ -547,7 +548,8 @@ __device__ __forceinline__ void rows_out(float* __restrict__ dst, int rows, int 
 }
 
 // Training forward: a Gaussian's fp32 coefficients are read once, rounded to codes (kept for the
-// backward), read back and evaluated.  The blocks that the degree touches are rounded whole, so a
+// backward), read back and evaluated.  Bound by memory: 1M Gaussians at degree 3 with 4 views (282 MB) 52 us,
+// 5.4 TB/s.  The blocks that the degree touches are rounded whole, so a
 // code does not depend on the degree.
 template <int DEG, bool NT, bool NT_COLOR>
 __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, const float* __restrict__ features,
@@ -614,7 +616,8 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_quantize(ShArgs a, con
 // One thread per Gaussian, all views; the features' gradient rows leave through LDS.  Which
 // channels take part comes from the forward's mask, so the constant coefficients (whose basis value
 // has no slope) are not read.
-// WANT_F: dfeatures is wanted (else at most its first coefficient, ddc).
+// WANT_F: dfeatures is wanted (else at most its first coefficient, ddc).  Bound by memory: 1M Gaussians at
+// degree 3 with 4 views (294 MB) 49 us, 6.0 TB/s.
 template <int DEG, bool WANT_F, bool NT>
 __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, const uint8_t* __restrict__ mask,
                                                                    const float* __restrict__ dcolors,
@@ -682,6 +685,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, con
     }
 }
 
+// Bound by memory, 12 bytes a row; one thread each (a strided column of a gradient has nothing wide to load).
 __global__ void __launch_bounds__(CP_THREADS) k_accumulate_weights(int P, const float* __restrict__ w,
                                                                    long long stride, float decay,
                                                                    float* __restrict__ acc) {
@@ -856,6 +860,8 @@ __device__ __forceinline__ KeepSel keep_small_pass(const uint32_t (&key)[16], in
     return {(st.prefix << (PASS == 2 ? 10 : 11)) | b.prefix, b.need, b.count};
 }
 
+// Bound by latency: one load of the keys, two or three rounds of LDS counters and scans behind it (10k rows
+// 8.6 us; with a barrier more on each side of every step 10).
 __global__ void __launch_bounds__(KEEP_SMALL_THREADS) k_keep_small(KeepArgs a, const float* __restrict__ w,
                                                                    int* __restrict__ ids) {
     // a part for each pass: no barrier between one pass's last reads and the next one's first writes
