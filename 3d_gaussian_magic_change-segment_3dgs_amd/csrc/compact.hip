@@ -703,7 +703,6 @@ __global__ void __launch_bounds__(CP_THREADS) k_accumulate_weights(int P, const 
 // larger groups take a launch per pass, the last of which also counts for each tile what the kernel
 // that writes the ids needs: what is read, 4 bytes a row and pass from the caches, is less than what
 // the launches and their dependences cost (five launches; 1M rows 26 us, with a sixth for the counts 29).
-// Weights that are all equal queue at one counter: 1M rows 33 us.
 constexpr int KEEP_TILE = CP_THREADS * 16;  // rows a block holds at once
 constexpr int KEEP_BINS = 2048;
 constexpr int KEEP_SMALL_THREADS = 1024, KEEP_SMALL = KEEP_SMALL_THREADS * 16;
@@ -811,15 +810,22 @@ __device__ __forceinline__ KeepSel find_bin(const uint32_t* hist, uint32_t need,
     return *s_out;
 }
 
-__device__ __forceinline__ void keep_add(uint32_t* h, uint32_t d, bool in) {
-    if (in) atomicAdd(&h[d], 1u);
+// A thread's N keys are all the same: they are added as one (adds to one counter queue, and equal
+// weights are common: 10k rows of zeros 34 -> 10 us, 1M 33 -> 27, 45M 577 -> 179; different ones cost 0.2 more).
+template <int N>
+__device__ __forceinline__ bool keep_flat(const uint32_t (&key)[N], bool all_in) {
+    uint32_t x = 0;
+#pragma unroll
+    for (int k = 1; k < N; ++k) x |= key[k] ^ key[0];
+    return x == 0 && all_in;
 }
 
-// Keys [i, i + 16) of rows below `end` (0 behind it).
-__device__ __forceinline__ void keep_load16(const float* __restrict__ w, long long i, long long end, uint32_t (&key)[16]) {
-    v4a v[4];
+// Keys [i, i + N) of rows below `end` (0 behind it).
+template <int N>
+__device__ __forceinline__ void keep_load(const float* __restrict__ w, long long i, long long end, uint32_t (&key)[N]) {
+    v4a v[N / 4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < N / 4; ++q) {
         v[q] = v4a{0.0f, 0.0f, 0.0f, 0.0f};
         if (i + 4 * q + 4 <= end) {
             v[q] = *reinterpret_cast<const v4a*>(w + i + 4 * q);
@@ -830,7 +836,7 @@ __device__ __forceinline__ void keep_load16(const float* __restrict__ w, long lo
         }
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < N / 4; ++q) {
         key[4 * q] = keep_key(v[q].x); key[4 * q + 1] = keep_key(v[q].y);
         key[4 * q + 2] = keep_key(v[q].z); key[4 * q + 3] = keep_key(v[q].w);
     }
@@ -846,22 +852,25 @@ __device__ __forceinline__ bool keep_digit(uint32_t key, uint32_t prefix, uint32
 __device__ __forceinline__ bool keep_early(KeepSel st) { return st.count == st.need && st.prefix > 0; }
 
 // One pass over the keys of a small group: the digits found before it -> one more.
-template <int PASS>
-__device__ __forceinline__ KeepSel keep_small_pass(const uint32_t (&key)[16], int n, KeepSel st, uint32_t* h,
+template <int PASS, int N>
+__device__ __forceinline__ KeepSel keep_small_pass(const uint32_t (&key)[N], bool flat, int n, KeepSel st, uint32_t* h,
                                                    uint32_t* s_wave, KeepSel* s_out) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
+    for (int k = 0; k < N; ++k) {
         uint32_t d;
-        const bool in = keep_digit<PASS>(key[k], st.prefix, d) && (int)threadIdx.x * 16 + k < n;
-        keep_add(h, d, in);
+        const bool in = keep_digit<PASS>(key[k], st.prefix, d) && (int)threadIdx.x * N + k < n;
+        if (in && (k == 0 || !flat)) atomicAdd(&h[d], flat ? (uint32_t)N : 1u);
     }
     __syncthreads();
     const KeepSel b = find_bin<KEEP_SMALL_THREADS>(h, st.need, s_wave, s_out);
     return {(st.prefix << (PASS == 2 ? 10 : 11)) | b.prefix, b.need, b.count};
 }
 
-// Bound by latency: one load of the keys, two or three rounds of LDS counters and scans behind it (10k rows
-// 8.6 us; with a barrier more on each side of every step 10).
+// Bound by latency: one load of the keys, two or three rounds of LDS counters and scans behind it.  N keys a
+// thread, as few as the largest group allows, so that all 16 waves share the work: 1000 rows 4.0 us (with 16 a
+// thread 8.0), 4000 4.5 (7.0), 10k 7.5 (8.5).  More than 16 are no gain over the launches of the large way (32k
+// rows 25 us, 17 there).
+template <int N>
 __global__ void __launch_bounds__(KEEP_SMALL_THREADS) k_keep_small(KeepArgs a, const float* __restrict__ w,
                                                                    int* __restrict__ ids) {
     // a part for each pass: no barrier between one pass's last reads and the next one's first writes
@@ -869,32 +878,33 @@ __global__ void __launch_bounds__(KEEP_SMALL_THREADS) k_keep_small(KeepArgs a, c
     __shared__ uint32_t s_wave[4][KEEP_SMALL_THREADS / 64];
     __shared__ KeepSel s_out[3];
     const KeepGroup G = a.g[blockIdx.x];
-    const int n = G.old_end - G.begin, first = threadIdx.x * 16;
+    const int n = G.old_end - G.begin, first = threadIdx.x * N;
     if (G.pick > 0) {  // the whole block
-        uint32_t key[16];
-        keep_load16(w, (long long)G.begin + first, G.old_end, key);
+        uint32_t key[N];
+        keep_load(w, (long long)G.begin + first, G.old_end, key);
         for (int k = threadIdx.x; k < 3 * KEEP_BINS; k += KEEP_SMALL_THREADS) h[0][k] = 0u;
         __syncthreads();
+        const bool flat = keep_flat(key, first + N <= n);
         KeepSel st = {0u, (uint32_t)G.pick, 0u};
-        st = keep_small_pass<0>(key, n, st, h[0], s_wave[0], &s_out[0]);
-        st = keep_small_pass<1>(key, n, st, h[1], s_wave[1], &s_out[1]);
+        st = keep_small_pass<0>(key, flat, n, st, h[0], s_wave[0], &s_out[0]);
+        st = keep_small_pass<1>(key, flat, n, st, h[1], s_wave[1], &s_out[1]);
         if (keep_early(st)) {
             st.prefix = (st.prefix << 10) - 1;
             st.need = 0;
         } else {
-            st = keep_small_pass<2>(key, n, st, h[2], s_wave[2], &s_out[2]);
+            st = keep_small_pass<2>(key, flat, n, st, h[2], s_wave[2], &s_out[2]);
         }
         uint32_t gt = 0, eq = 0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
+        for (int k = 0; k < N; ++k) {
             gt += first + k < n && key[k] > st.prefix;
             eq += first + k < n && key[k] == st.prefix;
         }
-        const uint32_t before = block_scan_excl<KEEP_SMALL_THREADS>(gt | eq << 16, s_wave[3]);  // at most 16384 each
+        const uint32_t before = block_scan_excl<KEEP_SMALL_THREADS>(gt | eq << 16, s_wave[3]);  // at most KEEP_SMALL < 65536 each
         gt = before & 0xFFFFu;
         eq = before >> 16;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
+        for (int k = 0; k < N; ++k) {
             if (first + k < n) {
                 const bool up = key[k] > st.prefix, tie = key[k] == st.prefix;
                 if (up || (tie && eq < st.need)) ids[G.out + gt + (eq < st.need ? eq : st.need)] = G.begin + first + k;
@@ -941,23 +951,24 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_hist(KeepArgs a, KeepWs ws,
     uint32_t key[16];
     const int rounds = MANY ? a.rounds : 1;
     long long base = G.begin + (long long)(tile - G.tile0) * rounds * KEEP_TILE + threadIdx.x * 16;
-    keep_load16(w, base, G.old_end, key);
+    keep_load(w, base, G.old_end, key);
     for (int k = threadIdx.x; k < BINS; k += CP_THREADS) h[k] = 0u;
     const KeepSel st = keep_state<PASS>(a, ws, g, tile, s_wave[0], &s_out);
     __syncthreads();
     const bool early = LAST && keep_early(st);
     uint32_t above = 0;
     for (int round = 1;; ++round) {
+        const bool flat = keep_flat(key, base + 16 <= G.old_end);
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
             uint32_t d;
             const bool in = base + k < G.old_end, same = keep_digit<PASS>(key[k], st.prefix, d);
             if constexpr (LAST) above += in && (key[k] >> 10 > st.prefix || (same && early));
-            keep_add(h, d, in && same && !early);
+            if (in && same && !early && (k == 0 || !flat)) atomicAdd(&h[d], flat ? 16u : 1u);
         }
         base += KEEP_TILE;
         if (!MANY || round == rounds || base - threadIdx.x * 16 >= G.old_end) break;  // the whole block
-        keep_load16(w, base, G.old_end, key);
+        keep_load(w, base, G.old_end, key);
     }
     if constexpr (LAST) {
         const uint32_t before = block_scan_excl<CP_THREADS>(above, s_wave[1]);
@@ -994,7 +1005,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
     if (G.pick > 0 && base < G.old_end) {  // the whole block
         long long first = base + threadIdx.x * 16;
         uint32_t key[16];
-        keep_load16(w, first, G.old_end, key);
+        keep_load(w, first, G.old_end, key);
         KeepSel st = ws.sel[g * 3 + 1];
         if (threadIdx.x == 0) s_gt = s_eq = 0;
         uint2 sum = {0u, 0u};
@@ -1018,7 +1029,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
             atomicAdd(&s_gt, sum.x);
             atomicAdd(&s_eq, sum.y);
         }
-        uint32_t gt0 = 0, eq0 = 0;  // rows above / equal to T before this round's
+        uint32_t gt0 = 0, eq0 = 0;  // rows above / equal to T before this piece
         for (int round = 1;; ++round) {
             uint32_t both = 0;
 #pragma unroll
@@ -1029,7 +1040,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
                 gt0 = s_gt;
                 eq0 = s_eq;
             }
-            const uint32_t ties = eq0 < st.need ? st.need - eq0 : 0u;  // left for this round
+            const uint32_t ties = eq0 < st.need ? st.need - eq0 : 0u;  // left for this piece
             uint32_t gt = before & 0xFFFFu, eq = before >> 16;
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
@@ -1043,7 +1054,7 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
             if (threadIdx.x == CP_THREADS - 1) s_n = gt | eq << 16;  // at most KEEP_TILE = 4096 of each
             first += KEEP_TILE;
             const bool more = MANY && round < rounds && first - threadIdx.x * 16 < G.old_end;  // the whole block
-            if (more) keep_load16(w, first, G.old_end, key);
+            if (more) keep_load(w, first, G.old_end, key);
             __syncthreads();
             gt = s_n & 0xFFFFu;
             eq = s_n >> 16;
@@ -1312,7 +1323,11 @@ GSR_API int gsr_keep_heaviest(int P, const float* weights, int n_groups, const g
     if (!weights || !ids || (!ws && P > KEEP_SMALL)) return set_error("[gsr] gsr_keep_heaviest: null buffer");
     hipStream_t st = (hipStream_t)stream;
     if (most <= KEEP_SMALL) {
-        k_keep_small<<<a.n, KEEP_SMALL_THREADS, 0, st>>>(a, weights, ids);
+        const int each = (most + KEEP_SMALL_THREADS - 1) / KEEP_SMALL_THREADS;  // keys a thread
+        if (each <= 4) k_keep_small<4><<<a.n, KEEP_SMALL_THREADS, 0, st>>>(a, weights, ids);
+        else if (each <= 8) k_keep_small<8><<<a.n, KEEP_SMALL_THREADS, 0, st>>>(a, weights, ids);
+        else if (each <= 12) k_keep_small<12><<<a.n, KEEP_SMALL_THREADS, 0, st>>>(a, weights, ids);
+        else k_keep_small<16><<<a.n, KEEP_SMALL_THREADS, 0, st>>>(a, weights, ids);
         return launched("keep_heaviest");
     }
     const KeepWs w = keep_ws(ws, keep_tiles((size_t)P));

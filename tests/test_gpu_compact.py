@@ -390,6 +390,18 @@ def test_keep_heaviest_groups():
     check_keep(w[:5000].view(5000, 1), 77)  # [P, 1], as the model holds them
 
 
+@pytest.mark.parametrize("n", [4100, 8191, 8192, 8193, 12_287, 12_288, 12_289])
+def test_keep_heaviest_runs_of_equal_weights(n):
+    """Runs that fill a thread's keys or end inside them, at the sizes where a thread takes more."""
+    g = gen(n)
+    for run in (4, 7, 16, 1000):
+        w = torch.exp(torch.randn(n // run + 1, generator=g)).repeat_interleave(run)[:n].contiguous()
+        for budget in (run, n // 2, n // 2 + 1, n - 1):
+            check_keep(w, budget)
+            check_keep(w, budget, recent=run // 2)
+    check_keep(torch.full((n,), float("nan")), n // 3)
+
+
 @pytest.mark.parametrize("kind", ["heavy", "equal", "whole"])
 def test_keep_heaviest_of_many_rows(kind):
     """9M rows (a block takes two pieces of a tile) and 17M (three): in one group, and in groups of unequal size whose
