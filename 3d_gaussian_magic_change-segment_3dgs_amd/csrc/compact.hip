@@ -18,7 +18,7 @@ __host__ __device__ inline int mx_words(int K) { return (K + 7) / 8; }
 __host__ __device__ inline int mx_blocks(int K) { return (K + GSR_MX_BLOCK - 1) / GSR_MX_BLOCK; }
 
 // How the units of a row of a streamed tensor (R rows of `units`) go to blocks of `span`
-// lanes: whole rows where a row fits, so that no lane divides (units 12 of a 1024 span:
+// lanes: whole rows where a row fits, so that no lane divides (units 9 of a 768 span:
 // 85 rows, 99.6 % of the lanes); pieces of a row otherwise.
 struct Tiling {
     int units, rows;  // rows a block (0: pieces)
@@ -1071,12 +1071,16 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
 
 // ------------------------------------------------------------------------ rows --
 // A copy: K rows of each tensor read and written once, bound by memory.  A block moves
-// TAKE_SPAN units of one tensor's output, a unit being 16 bytes where the rows are whole
-// float4s (the features, 48 of a Gaussian's 61 floats, and the rotations), else 4.  Loads and
-// wide stores pass by the caches: every line is wanted by one instruction (1M rows of 732 bytes
-// kept at 70 %: 215 us with temporal ones, 198 so, 5.2 TB/s).
+// TAKE_SPAN units of one tensor's output, a unit being 16 bytes where the rows are whole and aligned
+// float4s (the features, 48 of a Gaussian's 61 floats, and the rotations), else the largest of 12, 8 and
+// 4 that a row is made of (with 4 for all of those, their blocks were 40 % of the launch for 15 % of the
+// bytes).  Loads and stores of 16 and 12 bytes pass by the caches: every line is wanted by one
+// instruction.  1M rows of 732 bytes kept at 70 %: 181 us, 5.7 TB/s of what has to move; with units of 16
+// and 4 bytes only 196, with temporal accesses 215.  Narrow rows cost the lines of their dropped neighbours too.
 constexpr int TAKE_MAX = 32;    // tensors a launch
-constexpr int TAKE_PER = 4;     // units a thread: their ids, then their values, are in flight together
+// Units a thread: their ids, then their values, are in flight together.  3: a block is 64 rows of 192 bytes,
+// whole cache lines (2: 184 us, 4: 182, 8: 197).
+constexpr int TAKE_PER = 3;
 constexpr int TAKE_SPAN = CP_THREADS * TAKE_PER;
 struct TakeTensor {
     const void* src;
@@ -1092,10 +1096,38 @@ struct TakeArgs {
 };
 
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
-template <typename V>
+template <int U>
+struct TakeUnit {
+    uint32_t w[U];
+};
+template <int U>
+__device__ __forceinline__ TakeUnit<U> take_load(const uint32_t* p) {
+    TakeUnit<U> v;
+    if constexpr (U == 4) {
+        const u4v q = __builtin_nontemporal_load(reinterpret_cast<const u4v*>(p));
+        v.w[0] = q.x; v.w[1] = q.y; v.w[2] = q.z; v.w[3] = q.w;
+    } else {
+#pragma unroll
+        for (int k = 0; k < U; ++k) v.w[k] = __builtin_nontemporal_load(p + k);
+    }
+    return v;
+}
+template <int U>
+__device__ __forceinline__ void take_store(uint32_t* p, const TakeUnit<U>& v) {
+    if constexpr (U == 4) {
+        __builtin_nontemporal_store(u4v{v.w[0], v.w[1], v.w[2], v.w[3]}, reinterpret_cast<u4v*>(p));
+    } else {
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if constexpr (U == 3) __builtin_nontemporal_store(v.w[k], p + k);
+            else p[k] = v.w[k];
+        }
+    }
+}
+template <int U>
 __device__ __forceinline__ void take_block(const TakeTensor& t, uint32_t block, const int* __restrict__ ids) {
-    const V* src = static_cast<const V*>(t.src);
-    V* dst = static_cast<V*>(t.dst);
+    const uint32_t* src = static_cast<const uint32_t*>(t.src);
+    uint32_t* dst = static_cast<uint32_t*>(t.dst);
     long long to[TAKE_PER], from[TAKE_PER];
 #pragma unroll
     for (int k = 0; k < TAKE_PER; ++k) {
@@ -1103,22 +1135,20 @@ __device__ __forceinline__ void take_block(const TakeTensor& t, uint32_t block, 
         int unit;
         to[k] = from[k] = -1;
         if (tiling_place<TAKE_SPAN>(t.t, block, k * CP_THREADS + threadIdx.x, t.K, row, unit)) {
-            to[k] = row * t.t.units + unit;
+            to[k] = (row * t.t.units + unit) * U;
             const int id = ids[row];
-            if ((unsigned)id < (unsigned)t.rows) from[k] = (long long)id * t.t.units + unit;
+            if ((unsigned)id < (unsigned)t.rows) from[k] = ((long long)id * t.t.units + unit) * U;
         }
     }
-    V v[TAKE_PER];
-#pragma unroll
-    for (int k = 0; k < TAKE_PER; ++k) v[k] = from[k] >= 0 ? __builtin_nontemporal_load(src + from[k]) : V{};
+    TakeUnit<U> v[TAKE_PER] = {};
 #pragma unroll
     for (int k = 0; k < TAKE_PER; ++k)
-        if (to[k] >= 0) {
-            if constexpr (sizeof(V) == 16) __builtin_nontemporal_store(v[k], dst + to[k]);
-            else dst[to[k]] = v[k];
-        }
+        if (from[k] >= 0) v[k] = take_load<U>(src + from[k]);
+#pragma unroll
+    for (int k = 0; k < TAKE_PER; ++k)
+        if (to[k] >= 0) take_store<U>(dst + to[k], v[k]);
     if (t.pad > 0 && block == t.blocks - 1) {  // the words behind the last row
-        uint32_t* tail = reinterpret_cast<uint32_t*>(dst + (long long)t.K * t.t.units);
+        uint32_t* tail = dst + (long long)t.K * t.t.units * U;
         for (int k = threadIdx.x; k < t.pad; k += CP_THREADS) tail[k] = 0u;
     }
 }
@@ -1132,8 +1162,10 @@ __global__ void __launch_bounds__(CP_THREADS) k_take_rows(TakeArgs a, const int*
     }
     const TakeTensor t = a.t[lo];
     const uint32_t block = blockIdx.x - t.block0;
-    if (t.vec == 4) take_block<u4v>(t, block, ids);
-    else take_block<uint32_t>(t, block, ids);
+    if (t.vec == 4) take_block<4>(t, block, ids);
+    else if (t.vec == 3) take_block<3>(t, block, ids);
+    else if (t.vec == 2) take_block<2>(t, block, ids);
+    else take_block<1>(t, block, ids);
 }
 
 unsigned grid_for(long long items, long long cap) {
@@ -1381,11 +1413,12 @@ GSR_API int gsr_take_rows(int K, const int* ids, int n, const gsr_rows* tensors,
         for (int k = k0; k < n && k < k0 + TAKE_MAX; ++k) {
             const gsr_rows& q = tensors[k];
             const bool wide = q.width % 4 == 0 && ((uintptr_t)q.src | (uintptr_t)q.dst) % 16 == 0;
+            const int unit = wide ? 4 : q.width % 3 == 0 ? 3 : q.width % 2 == 0 ? 2 : 1;  // words
             if ((long long)K * q.width + q.pad == 0) continue;
-            const Tiling t = tiling(std::max(1, wide ? q.width / 4 : q.width), TAKE_SPAN);
+            const Tiling t = tiling(std::max(1, q.width / unit), TAKE_SPAN);
             const int rows = q.width > 0 ? K : 0;
             const long long nb = std::max(1LL, tiling_blocks(t, rows, TAKE_SPAN));
-            a.t[a.n++] = {q.src, q.dst, t, rows, q.rows, wide ? 4 : 1, q.pad, (uint32_t)blocks, (uint32_t)nb};
+            a.t[a.n++] = {q.src, q.dst, t, rows, q.rows, unit, q.pad, (uint32_t)blocks, (uint32_t)nb};
             blocks += nb;
             if (blocks >= (1LL << 31)) return set_error("[gsr] gsr_take_rows: too many rows in one call");
         }

@@ -491,6 +491,23 @@ def test_take_rows_of_ids_outside():
     assert torch.equal(y[0], x[3]) and torch.equal(y[4], x[0]) and (y[1:4] == 0).all() and (z == 0).all()
 
 
+@pytest.mark.parametrize("width", [6, 9, 10, 14, 15, 16, 27, 30, 768, 770, 2304, 2306, 2307, 2308])
+def test_take_rows_of_every_unit(width):
+    """Rows of 16-, 12-, 8- and 4-byte units, from memory that starts at any word and to memory that does."""
+    import gsr_train as G
+    K, P = 1000, 700
+    ids = torch.randint(-2, P + 2, (K,), generator=gen(width), dtype=torch.int32).to(DEV)
+    inside = ((ids >= 0) & (ids < P)).view(K, 1)
+    for lead in range(4):
+        x = torch.randn(P * width + lead, generator=gen(3)).to(DEV)[lead:].view(P, width)
+        want = torch.where(inside, x[ids.clamp(0, P - 1).long()], torch.zeros((), device=DEV))
+        assert torch.equal(G.take_rows(ids, [x])[0], want)
+        buf = torch.full((K * width + lead + 1,), 9.0, device=DEV)
+        out = buf[lead:-1].view(K, width)
+        G.take_rows(ids, [x], out=[out])
+        assert torch.equal(out, want) and (buf[:lead] == 9).all() and buf[-1] == 9
+
+
 def test_take_rows_wide_and_padded():
     """Rows wider than a block's span, and the words behind a destination's last row."""
     from gsr_train import compact as T
