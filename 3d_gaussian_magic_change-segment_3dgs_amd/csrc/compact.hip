@@ -483,9 +483,10 @@ __device__ __forceinline__ void wave_lds_wait() { asm volatile("s_waitcnt lgkmcn
 
 // With NT the rows pass by the caches: what those hold of a tensor that does not fit them is gone
 // before its next reader comes, and was in the way of other data until then.  Loads of 192 MB of
-// features (1M Gaussians, one view): forward 50 -> 43 us; of 58 MB (300k): 14.0 -> 15.2, so not there.
+// features (1M Gaussians, one view): forward 43 -> 40 us, a step 86 -> 78; of 115 MB (600k, 8 views) a step 99 -> 86;
+// of 58 MB (300k): forward 14.0 -> 15.2, so not there.
 // Stores of the gradient: 192 MB, backward 49 -> 39 us; 58 MB and 8 views, 31 -> 24.
-constexpr long long NT_LOAD_BYTES = 128LL << 20, NT_STORE_BYTES = 32LL << 20;
+constexpr long long NT_LOAD_BYTES = 64LL << 20, NT_STORE_BYTES = 32LL << 20;
 template <bool NT>
 __device__ __forceinline__ void rows_in(const float* __restrict__ src, int rows, int F, float* lds, int lane) {
     if (F == 48) {
