@@ -361,7 +361,12 @@ def keep_heaviest(weights, budgets, groups=None, recent=0):
     P = weights.numel()
     if P >= 2 ** 31:
         raise RuntimeError("keep_heaviest: at most 2^31 - 1 weights")
-    plan = _keep_groups("keep_heaviest", P, budgets, groups, recent)
+    return _keep(weights, _keep_groups("keep_heaviest", P, budgets, groups, recent))
+
+
+def _keep(weights, plan):
+    """keep_heaviest of a finished plan (_keep_groups)."""
+    P = weights.numel()
     _on_gpu("keep_heaviest", weights)
     weights = weights.contiguous()
     if _HOST is not None:

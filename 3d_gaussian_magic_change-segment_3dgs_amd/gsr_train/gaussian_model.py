@@ -415,8 +415,11 @@ class GaussianModel:
         `contribution` stay, in order, with their moments and statistics; Gaussians in no group
         go.  The host does not wait for the device.  Returns (ids, groups): the old index of each
         Gaussian (int32 [P]) and the groups' new ranges."""
-        plan = _compact._keep_groups("evict", self.num_points, budget, groups, recent)
-        ids = _compact.keep_heaviest(self.contribution, budget, groups, recent)
+        P = self.num_points
+        if self.contribution.dtype != torch.float32 or self.contribution.numel() != P:
+            raise RuntimeError(f"evict: contribution must hold {P} float32 weights")
+        plan = _compact._keep_groups("evict", P, budget, groups, recent)
+        ids = _compact._keep(self.contribution, plan)
         opt = self.optimizer
         arenas = [self._arena.data] + ([opt.exp_avg, opt.exp_avg_sq] if opt is not None else [])
         spec, new = _compact.take_gaussians(self._spec, ids, arenas)
