@@ -3,7 +3,8 @@
 // functions, as gsr_train/compact.py does them over ctypes, with its checks and messages: small calls
 // are bound by the host (10k Gaussians: colours 18 us through Python and ctypes, 3 us on the GPU).
 #include <torch/extension.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
@@ -110,6 +111,25 @@ void keep(AutogradContext* ctx, const at::Tensor& xyz, const at::Tensor& campos,
     ctx->saved_data["M"] = M;
 }
 
+// Stands for the derivative of a gradient.  Its edges lead to what the gradient is a function of, so that every
+// backward pass towards one of those, grad() of a single input too, comes through here and is refused.
+struct NoSecondDerivative : torch::autograd::Node {
+    variable_list apply(variable_list&&) override {
+        throw std::runtime_error("sh_colors: trying to differentiate twice (the colours are once_differentiable)");
+    }
+    std::string name() const override { return "NoSecondDerivative"; }
+};
+
+void once_differentiable(at::Tensor& gradient, const std::vector<torch::autograd::Edge>& of) {
+    torch::autograd::edge_list edges;
+    for (const auto& e : of)
+        if (e.is_valid()) edges.push_back(e);
+    if (!gradient.defined() || edges.empty()) return;  // a constant
+    std::shared_ptr<torch::autograd::Node> node(new NoSecondDerivative, torch::autograd::deleteNode);
+    node->set_next_edges(std::move(edges));
+    torch::autograd::set_history(gradient, node);
+}
+
 // The gradients wanted of (dxyz, ddc or dfeatures); a second derivative is refused when it is taken.
 variable_list gradients(AutogradContext* ctx, const at::Tensor& g_in, bool features) {
     const auto sv = ctx->get_saved_variables();
@@ -119,7 +139,6 @@ variable_list gradients(AutogradContext* ctx, const at::Tensor& g_in, bool featu
     const uint8_t* scales = apart ? sv[3].data_ptr<uint8_t>() : codes.data_ptr<uint8_t>() + P * 4 * words(3 * (M - 1));
     const uint8_t* mask = apart ? sv[4].data_ptr<uint8_t>() : scales + P * blocks(3 * (M - 1));
     Guard guard(xyz.device());
-    const bool twice = at::GradMode::is_enabled() && g_in.requires_grad();
     variable_list out(2);
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -134,15 +153,19 @@ variable_list gradients(AutogradContext* ctx, const at::Tensor& g_in, bool featu
                                          out[0].defined() ? out[0].data_ptr<float>() : nullptr,
                                          features ? nullptr : second, features ? second : nullptr, cur_stream()));
     }
-    if (twice) {
-        for (int k = 0; k < 2; ++k)
-            if (out[k].defined()) {
-                auto err = std::make_shared<torch::autograd::DelayedError>(
-                    "trying to differentiate twice a function that was marked with @once_differentiable", 1);
-                at::Tensor v = out[k].detach();
-                v.set_requires_grad(true);
-                out[k] = (*err)({v})[0];
-            }
+    if (at::GradMode::is_enabled()) {
+        // dxyz is a function of the upstream gradient, the positions and the coefficients above the constant one (and 0
+        // at degree 0); ddc is one of the upstream gradient alone, dfeatures of the positions too (straight through the
+        // rounding: not of the features).
+        const auto node = torch::autograd::get_current_node();
+        const torch::autograd::Edge up = torch::autograd::impl::gradient_edge(g_in);
+        const torch::autograd::Edge place = degree > 0 ? node->next_edge(0) : torch::autograd::Edge();
+        if (degree > 0) {
+            if (features) once_differentiable(out[0], {up, place, node->next_edge(1)});
+            else once_differentiable(out[0], {up, place});
+        }
+        if (features) once_differentiable(out[1], {up, place});
+        else once_differentiable(out[1], {up});
     }
     return out;
 }

@@ -21,7 +21,6 @@ captured backward pass would have to wait on the eager graph's stream."""
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _C
 from diff_gaussian_rasterization._C import MAX_VIEWS, _HOST
@@ -190,6 +189,26 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """A gradient as a function of `of`, whose derivative is refused."""
+
+    @staticmethod
+    def forward(ctx, gradient, *of):
+        return gradient.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("sh_colors: trying to differentiate twice (the colours are once_differentiable)")
+
+
+def _once(gradient, *of):
+    of = [t for t in of if t is not None and t.requires_grad]
+    if gradient is None or not of or not torch.is_grad_enabled():
+        return gradient
+    return _NoSecondDerivative.apply(gradient, *of)
+
+
+@torch.no_grad()
 def _backward(g, saved, degree, M, dxyz, ddc, dfeatures):
     xyz, campos, codes, scales, mask = saved
     P = xyz.shape[0]
@@ -215,13 +234,14 @@ class _ShColors(torch.autograd.Function):
         return colors
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
         xyz = ctx.saved_tensors[0]
         dxyz = torch.empty_like(xyz) if ctx.needs_input_grad[0] else None
         ddc = torch.empty_like(xyz) if ctx.needs_input_grad[1] else None
         _backward(g, ctx.saved_tensors, ctx.degree, ctx.M, dxyz, ddc, None)
-        return dxyz, ddc, None, None, None, None, None, None
+        if ctx.degree > 0:
+            dxyz = _once(dxyz, g, xyz)
+        return dxyz, _once(ddc, g), None, None, None, None, None, None
 
 
 class _ShColorsQuantized(torch.autograd.Function):
@@ -229,7 +249,7 @@ class _ShColorsQuantized(torch.autograd.Function):
     of the features for the backward are their codes, 26 bytes a Gaussian, and a byte a view."""
 
     @staticmethod
-    def forward(ctx, xyz, features, campos, degree, single):
+    def forward(ctx, xyz, features, campos, degree, single, history):
         P, M = features.shape[:2]
         K, V, dev = 3 * (M - 1), campos.shape[0], xyz.device
         codes = torch.empty((P, 4 * _words(K)), dtype=torch.uint8, device=dev)
@@ -239,11 +259,10 @@ class _ShColorsQuantized(torch.autograd.Function):
             _call(dev, _lib.gsr_sh_colors_quantize, P, V, degree, M, xyz.data_ptr(), features.data_ptr(),
                   campos.data_ptr(), codes.data_ptr(), scales.data_ptr(), mask.data_ptr(), colors.data_ptr())
         ctx.save_for_backward(xyz, campos, codes, scales, mask)
-        ctx.degree, ctx.M = degree, M
+        ctx.degree, ctx.M, ctx.history = degree, M, history
         return colors
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
         xyz = ctx.saved_tensors[0]
         dxyz = torch.empty_like(xyz) if ctx.needs_input_grad[0] else None
@@ -251,7 +270,9 @@ class _ShColorsQuantized(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             df = torch.empty((xyz.shape[0], ctx.M, 3), dtype=torch.float32, device=xyz.device)
         _backward(g, ctx.saved_tensors, ctx.degree, ctx.M, dxyz, None, df)
-        return dxyz, df, None, None, None
+        if ctx.degree > 0:  # (straight through the rounding: df is no function of the features)
+            return _once(dxyz, g, xyz, *ctx.history), _once(df, g, xyz), None, None, None, None
+        return dxyz, _once(df, g), None, None, None, None
 
 
 def _plain(a, b, c, degree):
@@ -269,7 +290,7 @@ def sh_colors(xyz, features_dc, rest, campos, degree):
     values, campos [3] -> colors [P, 3], or [V, 3] -> [V, P, 3].  Differentiable in xyz and
     features_dc (gradients summed over the views; campos gets none, nor do the codes); a
     channel that the clamp holds at zero gives no gradient, and a Gaussian at the camera
-    position itself none to xyz.  A features_dc of its own ([P, 3] contiguous) is read faster
+    position itself none to xyz.  Second derivatives are refused.  A features_dc of its own ([P, 3] contiguous) is read faster
     than a view of [P, M, 3] features, whose rows lie a cache line apart."""
     if _HOST is not None and isinstance(rest, MX4Rows) and _plain(xyz, features_dc, campos, degree):
         return _HOST.sh_colors(xyz, features_dc, rest.codes, rest.scales, rest.width, campos, degree)
@@ -308,8 +329,10 @@ def sh_colors_quantized(xyz, features, campos, degree):
         raise RuntimeError(f"{what}: features must have {xyz.shape[0]} rows (got {features.shape[0]})")
     _on_gpu(what, xyz, features=features, campos=campos)
     _capture_check(what, xyz, features)
+    # (an empty tensor that comes from the features, not their memory: what a gradient of the positions depends on)
+    history = (features[:0].clone(),) if torch.is_grad_enabled() and xyz.requires_grad else ()
     return _ShColorsQuantized.apply(xyz.contiguous(), features.contiguous(),
-                                    campos.detach().reshape(-1, 3).contiguous(), int(degree), campos.dim() == 1)
+                                    campos.detach().reshape(-1, 3).contiguous(), int(degree), campos.dim() == 1, history)
 
 
 # ---- eviction to a budget --------------------------------------------------------------------

@@ -28,3 +28,59 @@ def test_evict_with_weights_of_another_number():
     with pytest.raises(RuntimeError, match="contribution must hold 3000"):
         m.evict(100)
     assert m.num_points == 3000
+
+
+# ---- derivatives that there are none of -----------------------------------------------------------
+def test_second_derivatives_are_refused_under_a_linear_loss(monkeypatch):
+    """The first gradients depend on the inputs even where the upstream gradient is a constant: dxyz on xyz and on
+    the coefficients, dfeatures on xyz.  All of these are refused, by backward() and by grad() of one input."""
+    import gsr_train as G
+    xyz, f, cam, up = scene(40, 16, 2, 3)
+    xyz, f, cam, up = (t.to(DEV) for t in (xyz, f, cam, up))
+    rest = G.mx4_quantize(f.flatten(1)[:, 3:])
+
+    def fresh():
+        return [t.clone().requires_grad_() for t in (xyz, f, f[:, 0])]
+
+    def refused(run):
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            run()
+
+    for _ in both_routes(monkeypatch):
+        x, fg, dc = fresh()
+        first = lambda c, *of: torch.autograd.grad((c * up).sum(), of, create_graph=True)  # noqa: E731
+        trained = lambda: G.sh_colors_quantized(x, fg, cam, 3)  # noqa: E731
+        shown = lambda: G.sh_colors(x, dc, rest, cam, 3)  # noqa: E731
+        (gx,) = first(trained(), x)
+        refused(lambda: (gx.square().sum() + x.sum()).backward())
+        (gx,) = first(trained(), x)
+        refused(lambda: torch.autograd.grad(gx.square().sum() + x.sum(), x))
+        (gx,) = first(trained(), x)
+        refused(lambda: torch.autograd.grad(gx.sum() + fg.sum(), fg))
+        gx, gf = first(trained(), x, fg)
+        refused(lambda: torch.autograd.grad(gf.square().sum() + x.sum(), x))
+        (gx,) = first(shown(), x)
+        refused(lambda: (gx.square().sum() + x.sum()).backward())
+        (gx,) = first(shown(), x)
+        refused(lambda: torch.autograd.grad(gx.sum() + x.sum(), x))
+        # an upstream gradient that is a function of something
+        gd, = torch.autograd.grad(shown().square().sum(), dc, create_graph=True)
+        refused(lambda: torch.autograd.grad(gd.sum() + dc.sum(), dc))
+
+
+def test_first_gradients_that_are_constants_stay_usable(monkeypatch):
+    """What a second derivative would be zero of: the constants' gradient under a constant upstream gradient, the
+    features' one when the positions are fixed, everything at degree 0."""
+    import gsr_train as G
+    xyz, f, cam, up = (t.to(DEV) for t in scene(40, 16, 2, 3))
+    rest = G.mx4_quantize(f.flatten(1)[:, 3:])
+    for _ in both_routes(monkeypatch):
+        x, fg, dc = [t.clone().requires_grad_() for t in (xyz, f, f[:, 0])]
+        cases = [(G.sh_colors(x, dc, rest, cam, 3), dc, dc), (G.sh_colors_quantized(xyz, fg, cam, 3), fg, fg),
+                 (G.sh_colors_quantized(x, fg, cam, 0), fg, fg), (G.sh_colors_quantized(x, fg, cam, 0), x, x)]
+        for c, of, leaf in cases:
+            (want,) = torch.autograd.grad(c, of, up, retain_graph=True)
+            (g,) = torch.autograd.grad(c, of, up, create_graph=True)
+            assert torch.equal(g, want)
+            (one,) = torch.autograd.grad(g.square().sum() + leaf.sum(), leaf)
+            assert (one == 1).all()
