@@ -243,6 +243,12 @@ void check_capture(const char* what, const at::Tensor& a, const at::Tensor& b) {
     }
 }
 
+// A tangent on an input would be lost: refused, as autograd refuses it for a function without a forward-mode form.
+void check_forward(const char* what, std::initializer_list<const at::Tensor*> inputs) {
+    for (const at::Tensor* t : inputs)
+        if (t->_fw_grad(0).defined()) refuse(std::string(what) + ": there is no forward-mode derivative");
+}
+
 bool wanted(const char* what, const at::Tensor& a, const at::Tensor& b) {
     const bool yes = at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad());
     if (yes) check_capture(what, a, b);
@@ -288,6 +294,7 @@ at::Tensor sh_colors(const at::Tensor& xyz_, const at::Tensor& features_dc, cons
     check_device("sh_colors", "features_dc", features_dc, xyz_);
     check_device("sh_colors", "rest", codes, xyz_);
     check_device("sh_colors", "campos", campos_, xyz_);
+    check_forward("sh_colors", {&xyz_, &features_dc, &campos_});
     Guard guard(xyz_.device());
     const bool single = campos_.dim() == 1, grad = wanted("sh_colors", xyz_, features_dc);
     const at::Tensor xyz = xyz_.contiguous(), campos = views_of(campos_);
@@ -310,6 +317,7 @@ at::Tensor sh_colors_quantized(const at::Tensor& xyz_, const at::Tensor& feature
     check_gpu(what, xyz_);
     check_device(what, "features", features_, xyz_);
     check_device(what, "campos", campos_, xyz_);
+    check_forward(what, {&xyz_, &features_, &campos_});
     Guard guard(xyz_.device());
     const bool single = campos_.dim() == 1, grad = wanted(what, xyz_, features_);
     const at::Tensor xyz = xyz_.contiguous(), features = features_.contiguous(), campos = views_of(campos_);

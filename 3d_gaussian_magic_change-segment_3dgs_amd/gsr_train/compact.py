@@ -171,6 +171,11 @@ def _sh_check(what, xyz, campos, degree, M):
                            f"(degree {degree}, {M} coefficients)")
 
 
+def _forward_check(what, *tensors):
+    if any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what}: there is no forward-mode derivative")
+
+
 def _capture_check(what, *tensors):
     """The compiled binding looks for eager graphs of the same tensors, whose streams a captured backward pass
     must not touch; here there is no way to."""
@@ -290,8 +295,9 @@ def sh_colors(xyz, features_dc, rest, campos, degree):
     values, campos [3] -> colors [P, 3], or [V, 3] -> [V, P, 3].  Differentiable in xyz and
     features_dc (gradients summed over the views; campos gets none, nor do the codes); a
     channel that the clamp holds at zero gives no gradient, and a Gaussian at the camera
-    position itself none to xyz.  Second derivatives are refused.  A features_dc of its own ([P, 3] contiguous) is read faster
-    than a view of [P, M, 3] features, whose rows lie a cache line apart."""
+    position itself none to xyz.  Second derivatives and forward mode are refused.  A
+    features_dc of its own ([P, 3] contiguous) is read faster than a view of [P, M, 3] features,
+    whose rows lie a cache line apart."""
     if _HOST is not None and isinstance(rest, MX4Rows) and _plain(xyz, features_dc, campos, degree):
         return _HOST.sh_colors(xyz, features_dc, rest.codes, rest.scales, rest.width, campos, degree)
     if not isinstance(rest, MX4Rows) or rest.width % 3 or rest.width > 45:
@@ -305,6 +311,7 @@ def sh_colors(xyz, features_dc, rest, campos, degree):
     if rest.rows != P:
         raise RuntimeError(f"sh_colors: rest must have {P} rows (got {rest.rows})")
     _on_gpu("sh_colors", xyz, features_dc=features_dc, rest=rest, campos=campos)
+    _forward_check("sh_colors", xyz, features_dc, campos)
     _capture_check("sh_colors", xyz, features_dc)
     dc = features_dc.reshape(P, 3)
     if P and (dc.stride(1) != 1 or (P > 1 and dc.stride(0) < 3)):
@@ -328,6 +335,7 @@ def sh_colors_quantized(xyz, features, campos, degree):
     if features.shape[0] != xyz.shape[0]:
         raise RuntimeError(f"{what}: features must have {xyz.shape[0]} rows (got {features.shape[0]})")
     _on_gpu(what, xyz, features=features, campos=campos)
+    _forward_check(what, xyz, features, campos)
     _capture_check(what, xyz, features)
     # (an empty tensor that comes from the features, not their memory: what a gradient of the positions depends on)
     history = (features[:0].clone(),) if torch.is_grad_enabled() and xyz.requires_grad else ()

@@ -84,3 +84,28 @@ def test_first_gradients_that_are_constants_stay_usable(monkeypatch):
             assert torch.equal(g, want)
             (one,) = torch.autograd.grad(g.square().sum() + leaf.sum(), leaf)
             assert (one == 1).all()
+
+
+def test_forward_mode_is_refused(monkeypatch):
+    """A tangent on an input would be lost: no colours without it."""
+    import gsr_train as G
+    import torch.autograd.forward_ad as fw
+    xyz, f, cam, _ = (t.to(DEV) for t in scene(20, 4, 1, 8))
+    rest = G.mx4_quantize(f.flatten(1)[:, 3:])
+    dc = f[:, 0].contiguous()
+    for _ in both_routes(monkeypatch):
+        shown, trained = G.sh_colors(xyz, dc, rest, cam, 1), G.sh_colors_quantized(xyz, f, cam, 1)
+        with fw.dual_level():
+            dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+            for call in (lambda: G.sh_colors(dual(xyz), dc, rest, cam, 1), lambda: G.sh_colors(xyz, dual(dc), rest, cam, 1),
+                         lambda: G.sh_colors(xyz, dc, rest, dual(cam), 1),
+                         lambda: G.sh_colors_quantized(dual(xyz), f, cam, 1),
+                         lambda: G.sh_colors_quantized(xyz, dual(f), cam, 1),
+                         lambda: G.sh_colors_quantized(xyz, f, dual(cam), 1)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+            # other tensors of the level do not matter
+            assert torch.equal(G.sh_colors(xyz, dc, rest, cam, 1), shown)
+            assert torch.equal(G.sh_colors_quantized(xyz, f, cam, 1), trained)
