@@ -3,6 +3,8 @@
 // functions, as gsr_train/compact.py does them over ctypes, with its checks and messages: small calls
 // are bound by the host (10k Gaussians: colours 18 us through Python and ctypes, 3 us on the GPU).
 #include <torch/extension.h>
+#include <ATen/TracerMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
@@ -52,9 +54,20 @@ void check_device(const char* what, const char* name, const at::Tensor& t, const
         refuse(std::string(what) + ": " + name + " is on " + t.device().str() + ", expected " + first.device().str());
 }
 
+// A tracer would record the allocations and not the kernels: what it made would return uninitialised memory.
+bool jit_traced() { return at::tracer::impl::is_dispatch_enabled(); }
+bool fx_traced() {
+    using namespace c10::impl;
+    return TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value();
+}
+void check_traced(const char* what, bool traced = jit_traced() || fx_traced()) {
+    if (traced) refuse(std::string(what) + ": cannot be traced");
+}
+
 }  // namespace
 
 std::tuple<at::Tensor, at::Tensor> mx4_quantize(const at::Tensor& rows) {
+    check_traced("mx4_quantize");
     check_float("mx4_quantize", "x", rows);
     if (rows.dim() != 2) refuse("mx4_quantize: x must have shape (rows, values)");
     check_gpu("mx4_quantize", rows);
@@ -72,6 +85,7 @@ std::tuple<at::Tensor, at::Tensor> mx4_quantize(const at::Tensor& rows) {
 }
 
 at::Tensor mx4_dequantize(const at::Tensor& codes, const at::Tensor& scales, int64_t K) {
+    check_traced("MX4Rows.dequantize");
     Guard guard(codes.device());
     at::Tensor x = at::empty({codes.size(0), K}, like(codes, at::kFloat));
     if (x.numel())
@@ -279,6 +293,8 @@ at::Tensor views_of(const at::Tensor& campos) {
 
 at::Tensor sh_colors(const at::Tensor& xyz_, const at::Tensor& features_dc, const at::Tensor& codes,
                      const at::Tensor& scales, int64_t width, const at::Tensor& campos_, int64_t degree) {
+    if (jit_traced()) return {};  // the caller's Python function, which the tracer records as a whole
+    check_traced("sh_colors", fx_traced());
     if (width % 3 || width > 45) refuse("sh_colors: rest must be MX4Rows of 3 (M - 1) values, M of 1..16");
     const int64_t M = width / 3 + 1;
     check_sh("sh_colors", xyz_, campos_, degree, M);
@@ -307,6 +323,8 @@ at::Tensor sh_colors(const at::Tensor& xyz_, const at::Tensor& features_dc, cons
 at::Tensor sh_colors_quantized(const at::Tensor& xyz_, const at::Tensor& features_, const at::Tensor& campos_,
                                int64_t degree) {
     const char* what = "sh_colors_quantized";
+    if (jit_traced()) return {};  // (as sh_colors)
+    check_traced(what, fx_traced());
     check_float(what, "features", features_);
     if (features_.dim() != 3 || features_.size(2) != 3 || features_.size(1) < 1 || features_.size(1) > 16)
         refuse(std::string(what) + ": features must have shape (P, M, 3), M of 1..16");
@@ -327,6 +345,7 @@ at::Tensor sh_colors_quantized(const at::Tensor& xyz_, const at::Tensor& feature
 }
 
 at::Tensor keep_heaviest(const at::Tensor& weights, const std::vector<std::tuple<int, int, int, int>>& plan) {
+    check_traced("keep_heaviest");
     Guard guard(weights.device());
     std::vector<gsr_keep_group> g;
     int64_t n = 0;
@@ -348,6 +367,7 @@ at::Tensor keep_heaviest(const at::Tensor& weights, const std::vector<std::tuple
 // compact.py _take: the tensors' checks, the outputs where none are given, one gsr_take_rows.
 std::vector<at::Tensor> take_rows(const at::Tensor& ids, const std::vector<at::Tensor>& tensors,
                                   std::vector<at::Tensor> out, const std::vector<int>& pad, bool given) {
+    check_traced("take_rows");
     const int64_t K = ids.size(0);
     auto fine = [&](const at::Tensor& t) {
         return (t.scalar_type() == at::kFloat || t.scalar_type() == at::kInt) && t.dim() >= 1 && t.is_contiguous() &&

@@ -17,10 +17,13 @@ All tensors are float32 (ids int32, codes and scales uint8) on one GPU; a call u
 GPU's current stream, takes its workspace from torch's allocator and never waits for the
 device, so it can be captured into a graph.  A pass with gradients is captured forward and
 backward together, with no eager graph of the same leaves alive: that is refused, since the
-captured backward pass would have to wait on the eager graph's stream."""
+captured backward pass would have to wait on the eager graph's stream.  torch.jit.trace records
+sh_colors and sh_colors_quantized as calls of them; the other operators, and all of them under
+make_fx, refuse to be traced."""
 import ctypes
 
 import torch
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _C
 from diff_gaussian_rasterization._C import MAX_VIEWS, _HOST
@@ -74,6 +77,12 @@ def _on_gpu(what, first, **others):
             raise RuntimeError(f"{what}: {name} is on {t.device}, expected {first.device}")
 
 
+def _trace_check(what, jit=True):
+    """A tracer would record the allocations and not the kernels: what it made would return uninitialised memory."""
+    if (jit and torch._C._get_tracing_state() is not None) or get_proxy_mode() is not None:
+        raise RuntimeError(f"{what}: cannot be traced")
+
+
 def _call(device, fn, *args):
     """fn on `device` and its current stream."""
     with torch.cuda.device(device):
@@ -119,6 +128,7 @@ class MX4Rows:
         _on_gpu("MX4Rows.dequantize", self.codes)
         if _HOST is not None:
             return _HOST.mx4_dequantize(self.codes, self.scales, self.width)
+        _trace_check("MX4Rows.dequantize")
         x = torch.empty((self.rows, self.width), dtype=torch.float32, device=self.device)
         if x.numel():
             _call(self.device, _lib.gsr_mx4_dequantize, self.rows, self.width, self.codes.data_ptr(),
@@ -146,6 +156,7 @@ def mx4_quantize(x):
     if _HOST is not None and isinstance(x, torch.Tensor):
         codes, scales = _HOST.mx4_quantize(x)
     else:
+        _trace_check("mx4_quantize")
         _typed("mx4_quantize", x=x)
         if x.dim() != 2:
             raise RuntimeError("mx4_quantize: x must have shape (rows, values)")
@@ -299,7 +310,10 @@ def sh_colors(xyz, features_dc, rest, campos, degree):
     features_dc of its own ([P, 3] contiguous) is read faster than a view of [P, M, 3] features,
     whose rows lie a cache line apart."""
     if _HOST is not None and isinstance(rest, MX4Rows) and _plain(xyz, features_dc, campos, degree):
-        return _HOST.sh_colors(xyz, features_dc, rest.codes, rest.scales, rest.width, campos, degree)
+        colors = _HOST.sh_colors(xyz, features_dc, rest.codes, rest.scales, rest.width, campos, degree)
+        if colors is not None:  # (None under torch.jit.trace, which records the Python function below)
+            return colors
+    _trace_check("sh_colors", jit=False)
     if not isinstance(rest, MX4Rows) or rest.width % 3 or rest.width > 45:
         raise RuntimeError("sh_colors: rest must be MX4Rows of 3 (M - 1) values, M of 1..16")
     M = rest.width // 3 + 1
@@ -326,8 +340,11 @@ def sh_colors_quantized(xyz, features, campos, degree):
     model shows after `compact()`.  Differentiable in xyz and features; the gradient goes
     straight through the rounding, and coefficients above `degree` get zero."""
     if _HOST is not None and _plain(xyz, features, campos, degree):
-        return _HOST.sh_colors_quantized(xyz, features, campos, degree)
+        colors = _HOST.sh_colors_quantized(xyz, features, campos, degree)
+        if colors is not None:  # (as sh_colors)
+            return colors
     what = "sh_colors_quantized"
+    _trace_check(what, jit=False)
     _typed(what, features=features)
     if features.dim() != 3 or features.shape[2] != 3 or not 1 <= features.shape[1] <= 16:
         raise RuntimeError(f"{what}: features must have shape (P, M, 3), M of 1..16")
@@ -348,6 +365,7 @@ def sh_colors_quantized(xyz, features, campos, degree):
 def accumulate_weights(acc, weights, decay=1.0):
     """acc <- decay * acc + weights, in place: acc float32 contiguous of P values, weights
     float32 [P] of any stride (a column of a [P, 3] gradient)."""
+    _trace_check("accumulate_weights")
     _typed("accumulate_weights", acc=acc, weights=weights)
     P = acc.numel()
     if not acc.is_contiguous() or weights.dim() != 1 or weights.shape[0] != P:
@@ -397,6 +415,7 @@ def keep_heaviest(weights, budgets, groups=None, recent=0):
 
 def _keep(weights, plan):
     """keep_heaviest of a finished plan (_keep_groups)."""
+    _trace_check("keep_heaviest")
     P = weights.numel()
     _on_gpu("keep_heaviest", weights)
     weights = weights.contiguous()
@@ -433,6 +452,7 @@ def _take(ids, tensors, out, pad):
             return got if out is None else out
         except TypeError:  # something that is no tensor: refused below
             pass
+    _trace_check("take_rows")
     if out is None:
         out = [torch.empty((K,) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device) if isinstance(t, torch.Tensor)
                else None for t in tensors]

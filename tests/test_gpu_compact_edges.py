@@ -109,3 +109,59 @@ def test_forward_mode_is_refused(monkeypatch):
             # other tensors of the level do not matter
             assert torch.equal(G.sh_colors(xyz, dc, rest, cam, 1), shown)
             assert torch.equal(G.sh_colors_quantized(xyz, f, cam, 1), trained)
+
+
+# ---- tracing --------------------------------------------------------------------------------------
+def test_traced_colors_are_computed(monkeypatch):
+    """A traced call runs the operator on the new inputs (a recorded allocation without the kernel would be
+    uninitialised memory), with gradients."""
+    import gsr_train as G
+    xyz, f, cam, up = (t.to(DEV) for t in scene(200, 9, 2, 14))
+    other, f2, cam2, _ = (t.to(DEV) for t in scene(200, 9, 2, 15))
+    rest = G.mx4_quantize(f.flatten(1)[:, 3:])
+    for _ in both_routes(monkeypatch):
+        for trained in (True, False):
+            if trained:
+                fn = lambda x, c, k: G.sh_colors_quantized(x, c, k, 2)  # noqa: E731
+            else:
+                fn = lambda x, c, k: G.sh_colors(x, c[:, 0], rest, k, 2)  # noqa: E731
+            for grad in (False, True):
+                x, c = xyz.clone().requires_grad_(grad), f.clone().requires_grad_(grad)
+                traced = torch.jit.trace(fn, (x, c, cam), check_trace=False)
+                x, c = other.clone().requires_grad_(grad), f2.clone().requires_grad_(grad)
+                got, want = traced(x, c, cam2), fn(x, c, cam2)
+                assert torch.equal(got, want)
+                if grad:
+                    for a, b in zip(torch.autograd.grad(got, (x, c), up), torch.autograd.grad(want, (x, c), up)):
+                        assert torch.equal(a, b)
+
+
+def test_other_operators_refuse_to_be_traced(monkeypatch):
+    import gsr_train as G
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn(100, 45, generator=gen(1)).to(DEV)
+    w = torch.rand(100, generator=gen(2)).to(DEV)
+    ids = torch.arange(10, dtype=torch.int32, device=DEV)
+    rows = G.mx4_quantize(x)
+    xyz, f, cam, _ = (t.to(DEV) for t in scene(20, 4, 1, 8))
+    rest = G.mx4_quantize(f.flatten(1)[:, 3:])
+    calls = [(lambda t: G.mx4_quantize(t).codes, x), (lambda t: rows.dequantize() + t[:1], x),
+             (lambda t: G.keep_heaviest(t, 5), w), (lambda t: G.take_rows(ids, [t])[0], x)]
+    for _ in both_routes(monkeypatch):
+        for fn, arg in calls:
+            with pytest.raises(RuntimeError, match="traced"):
+                torch.jit.trace(fn, (arg,), check_trace=False)
+            with pytest.raises(RuntimeError, match="traced"):
+                make_fx(fn)(arg)
+        acc = torch.zeros(100, device=DEV)
+
+        def add(t):
+            G.accumulate_weights(acc, t)
+            return t + 0
+
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(add, (w,), check_trace=False)
+        assert (acc == 0).all()
+        for fn in (lambda t: G.sh_colors_quantized(t, f, cam, 1), lambda t: G.sh_colors(t, f[:, 0], rest, cam, 1)):
+            with pytest.raises(RuntimeError, match="traced"):
+                make_fx(fn)(xyz)
