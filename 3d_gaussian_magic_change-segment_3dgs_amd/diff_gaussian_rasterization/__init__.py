@@ -132,10 +132,11 @@ def rasterize_gaussians(
     raster_settings,
 ):
     s = raster_settings
-    if _C._HOST_AUTOGRAD is not None and not s.debug and not _SINKS:
+    if _C._HOST_AUTOGRAD is not None and not s.debug and not _SINKS and torch._C._get_tracing_state() is None:
         # the same autograd function in C++ (csrc/host_ext.cpp RasterizeFn): same outputs, saved
-        # state and gradients, without autograd's Python hops.  Debug mode (snapshot dumps) and
-        # forwards inside defer_sh_gradients take _RasterizeGaussians.
+        # state and gradients, without autograd's Python hops.  Debug mode (snapshot dumps),
+        # forwards inside defer_sh_gradients and torch.jit.trace (which records a call of the Python
+        # function, but of the C++ one only its allocations) take _RasterizeGaussians.
         device = means3D.device
         *out, num_rendered = _C._HOST_AUTOGRAD.rasterize(
             means3D, means2D, sh, colors_precomp, segments, opacities, scales, rotations, cov3Ds_precomp, s.bg,
