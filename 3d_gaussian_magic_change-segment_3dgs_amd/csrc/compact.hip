@@ -1178,7 +1178,7 @@ unsigned grid_for(long long items, long long cap) {
 constexpr int MAX_P = 0x7FFFFFFF - CP_THREADS;
 
 int check_rows(long long R, int K) {
-    if (R < 0 || K < 0 || K > (1 << 20) || (K > 0 && R > (1LL << 42) / K))  // (products of the two stay far from 2^63)
+    if (R < 0 || K < 0 || K > GSR_MAX_WIDTH || (K > 0 && R > (1LL << 42) / K))  // (products of the two stay far from 2^63)
         return set_error("[gsr] mx4: invalid number or width of rows");
     return 0;
 }
@@ -1382,7 +1382,7 @@ GSR_API int gsr_take_rows(int K, const int* ids, int n, const gsr_rows* tensors,
         return set_error("[gsr] gsr_take_rows: invalid arguments");
     for (int k = 0; k < n; ++k) {
         const gsr_rows& t = tensors[k];
-        if (t.width < 0 || t.width > (1 << 20) || t.rows < 0 || t.pad < 0)
+        if (t.width < 0 || t.width > GSR_MAX_WIDTH || t.rows < 0 || t.pad < 0)
             return set_error("[gsr] gsr_take_rows: invalid width or rows");
         const long long words = (long long)K * t.width;
         if ((words > 0 && t.rows > 0 && !t.src) || (words + t.pad > 0 && !t.dst))

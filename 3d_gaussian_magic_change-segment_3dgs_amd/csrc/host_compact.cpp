@@ -64,12 +64,18 @@ void check_traced(const char* what, bool traced = jit_traced() || fx_traced()) {
     if (traced) refuse(std::string(what) + ": cannot be traced");
 }
 
+// (the library takes a width as an int)
+void check_width(const char* what, int64_t K) {
+    if (K > GSR_MAX_WIDTH) refuse(std::string(what) + ": rows of more than 2^20 values");
+}
+
 }  // namespace
 
 std::tuple<at::Tensor, at::Tensor> mx4_quantize(const at::Tensor& rows) {
     check_traced("mx4_quantize");
     check_float("mx4_quantize", "x", rows);
     if (rows.dim() != 2) refuse("mx4_quantize: x must have shape (rows, values)");
+    if (rows.size(0)) check_width("mx4_quantize", rows.size(1));
     check_gpu("mx4_quantize", rows);
     Guard guard(rows.device());
     const bool apart = rows.numel() && ((rows.size(1) > 1 && rows.stride(1) != 1) ||
@@ -86,6 +92,8 @@ std::tuple<at::Tensor, at::Tensor> mx4_quantize(const at::Tensor& rows) {
 
 at::Tensor mx4_dequantize(const at::Tensor& codes, const at::Tensor& scales, int64_t K) {
     check_traced("MX4Rows.dequantize");
+    if (codes.size(0)) check_width("MX4Rows.dequantize", K);
+    check_gpu("MX4Rows.dequantize", codes);
     Guard guard(codes.device());
     at::Tensor x = at::empty({codes.size(0), K}, like(codes, at::kFloat));
     if (x.numel())
@@ -385,7 +393,7 @@ std::vector<at::Tensor> take_rows(const at::Tensor& ids, const std::vector<at::T
         if (!fine(t)) bad("tensors", n);
         int64_t width = 1;
         for (int64_t d = 1; d < t.dim(); ++d) width *= t.size(d);
-        if (width > (1 << 20)) refuse("take_rows: rows of more than 2^20 values");
+        check_width("take_rows", width);
         if (!given) {
             std::vector<int64_t> shape = t.sizes().vec();
             shape[0] = K;

@@ -32,6 +32,7 @@ _lib = _C._lib
 _vp, _i, _ll, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 
 MX_BLOCK = 32    # include/gsr_compact.h GSR_MX_BLOCK
+MAX_WIDTH = 1 << 20  # GSR_MAX_WIDTH
 MAX_GROUPS = 64  # GSR_KEEP_MAX_GROUPS
 
 
@@ -89,6 +90,11 @@ def _call(device, fn, *args):
         _C._check(fn(*args, _C._stream(device)))
 
 
+def _width_check(what, K):
+    if K > MAX_WIDTH:  # (the library takes a width as an int)
+        raise RuntimeError(f"{what}: rows of more than 2^20 values")
+
+
 def _words(K):
     return (K + 7) // 8
 
@@ -125,10 +131,12 @@ class MX4Rows:
 
     def dequantize(self):
         """The values the codes stand for, float32 [rows, width] (each is exact)."""
-        _on_gpu("MX4Rows.dequantize", self.codes)
         if _HOST is not None:
             return _HOST.mx4_dequantize(self.codes, self.scales, self.width)
         _trace_check("MX4Rows.dequantize")
+        if self.rows:
+            _width_check("MX4Rows.dequantize", self.width)
+        _on_gpu("MX4Rows.dequantize", self.codes)
         x = torch.empty((self.rows, self.width), dtype=torch.float32, device=self.device)
         if x.numel():
             _call(self.device, _lib.gsr_mx4_dequantize, self.rows, self.width, self.codes.data_ptr(),
@@ -160,6 +168,8 @@ def mx4_quantize(x):
         _typed("mx4_quantize", x=x)
         if x.dim() != 2:
             raise RuntimeError("mx4_quantize: x must have shape (rows, values)")
+        if x.shape[0]:
+            _width_check("mx4_quantize", x.shape[1])
         _on_gpu("mx4_quantize", x)
         if x.numel() and ((x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
             x = x.contiguous()
@@ -368,6 +378,8 @@ def accumulate_weights(acc, weights, decay=1.0):
     _trace_check("accumulate_weights")
     _typed("accumulate_weights", acc=acc, weights=weights)
     P = acc.numel()
+    if P >= 2 ** 31:
+        raise RuntimeError("accumulate_weights: at most 2^31 - 1 weights")
     if not acc.is_contiguous() or weights.dim() != 1 or weights.shape[0] != P:
         raise RuntimeError("accumulate_weights: acc must be contiguous and weights have shape (P,), P values each")
     _on_gpu("accumulate_weights", acc, weights=weights)
@@ -468,8 +480,7 @@ def _take(ids, tensors, out, pad):
         width = 1
         for d in t.shape[1:]:
             width *= d
-        if width > 1 << 20:
-            raise RuntimeError("take_rows: rows of more than 2^20 values")
+        _width_check("take_rows", width)
         table[n] = (t.data_ptr(), o.data_ptr(), width, t.shape[0], pad[n] if pad else 0)
     _on_gpu("take_rows", ids)
     if tensors:

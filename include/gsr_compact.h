@@ -28,6 +28,7 @@ extern "C" {
 #endif
 
 #define GSR_MX_BLOCK 32
+#define GSR_MAX_WIDTH (1 << 20) /* words of a row, K or width below */
 
 /* R rows of K floats, row i at x + i * row_stride -> codes, scales (codes 4-B aligned). */
 GSR_API int gsr_mx4_quantize(long long R, int K, const float* x, long long row_stride, uint32_t* codes,

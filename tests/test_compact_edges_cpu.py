@@ -1,0 +1,33 @@
+"""Compact-scene operators without a GPU: arguments at the edges of what a call takes (tests/test_compact_cpu.py has
+the ordinary refusals)."""
+import pytest
+import torch
+
+from test_compact_cpu import refused
+
+
+@pytest.fixture(params=["host", "ctypes"])
+def route(request, monkeypatch):
+    """Both host routes."""
+    from gsr_train import compact as T
+    if request.param == "host" and T._HOST is None:
+        pytest.skip("gsr_host not built from these sources (__graft_entry__.build())")
+    if request.param == "ctypes":
+        monkeypatch.setattr(T, "_HOST", None)
+    return request.param
+
+
+def test_sizes_that_do_not_fit_an_int_are_refused(route):
+    """Tensors without memory: what counts is that no size is cut to 32 bits on its way to the library."""
+    import gsr_train as G
+    meta = lambda *s, **k: torch.empty(*s, device="meta", **k)  # noqa: E731
+    for n in (2 ** 31, 2 ** 32 + 7):
+        refused(G.accumulate_weights, meta(n), meta(n), match="2\\^31")
+        refused(G.keep_heaviest, meta(n), 5, match="2\\^31")
+    for K in (2 ** 20 + 1, 2 ** 31, 2 ** 32 + 45):
+        refused(G.mx4_quantize, meta(1, K), match="2\\^20")
+        words, blocks = (K + 7) // 8, (K + 31) // 32
+        rows = G.MX4Rows(meta(1, 4 * words, dtype=torch.uint8), meta(1, blocks, dtype=torch.uint8), K)
+        refused(rows.dequantize, match="2\\^20")
+    refused(G.mx4_quantize, meta(3, 2 ** 20), match="GPU")  # the widest
+    refused(G.mx4_quantize, meta(0, 2 ** 21), match="GPU")  # nothing of any width
