@@ -408,6 +408,9 @@ std::vector<at::Tensor> take_rows(const at::Tensor& ids, const std::vector<at::T
         table.push_back({t.data_ptr(), out[n].data_ptr(), (int)width, (int)t.size(0), pad.empty() ? 0 : pad[n]});
     }
     if (!table.empty()) check(gsr_take_rows((int)K, ids.data_ptr<int>(), (int)table.size(), table.data(), cur_stream()));
+    if (given)  // a write that autograd has to know of
+        for (const at::Tensor& o : out)
+            if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
     return out;
 }
 

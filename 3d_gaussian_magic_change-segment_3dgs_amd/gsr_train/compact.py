@@ -90,6 +90,12 @@ def _call(device, fn, *args):
         _C._check(fn(*args, _C._stream(device)))
 
 
+def _written(t):
+    """Tells autograd of a write through the pointer."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _width_check(what, K):
     if K > MAX_WIDTH:  # (the library takes a width as an int)
         raise RuntimeError(f"{what}: rows of more than 2^20 values")
@@ -386,6 +392,7 @@ def accumulate_weights(acc, weights, decay=1.0):
     if P:
         _call(acc.device, _lib.gsr_accumulate_weights, P, weights.data_ptr(), weights.stride(0), float(decay),
               acc.data_ptr())
+        _written(acc)
 
 
 def _keep_groups(what, P, budgets, groups, recent):
@@ -465,6 +472,7 @@ def _take(ids, tensors, out, pad):
         except TypeError:  # something that is no tensor: refused below
             pass
     _trace_check("take_rows")
+    given = out is not None
     if out is None:
         out = [torch.empty((K,) + tuple(t.shape[1:]), dtype=t.dtype, device=t.device) if isinstance(t, torch.Tensor)
                else None for t in tensors]
@@ -485,6 +493,9 @@ def _take(ids, tensors, out, pad):
     _on_gpu("take_rows", ids)
     if tensors:
         _call(ids.device, _lib.gsr_take_rows, K, ids.data_ptr(), len(tensors), table)
+    if given:
+        for o in out:
+            _written(o)
     return out
 
 

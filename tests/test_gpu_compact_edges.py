@@ -165,3 +165,32 @@ def test_other_operators_refuse_to_be_traced(monkeypatch):
         for fn in (lambda t: G.sh_colors_quantized(t, f, cam, 1), lambda t: G.sh_colors(t, f[:, 0], rest, cam, 1)):
             with pytest.raises(RuntimeError, match="traced"):
                 make_fx(fn)(xyz)
+
+
+# ---- writes in place ------------------------------------------------------------------------------
+def test_writes_in_place_are_seen_by_autograd(monkeypatch):
+    """A tensor that another graph has saved cannot be written behind its back."""
+    import gsr_train as G
+    ids = torch.arange(5, dtype=torch.int32, device=DEV)
+    for _ in both_routes(monkeypatch):
+        x = torch.randn(5, 3, device=DEV).requires_grad_()
+        acc, out = torch.rand(5, device=DEV), torch.rand(5, 3, device=DEV)
+        loss = (x[:, 0] * acc).sum()
+        G.accumulate_weights(acc, torch.ones(5, device=DEV))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        loss = (x * out).sum()
+        G.take_rows(ids, [torch.rand(9, 3, device=DEV)], out=[out])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        # a refused call has written nothing
+        loss = (x * out).sum()
+        with pytest.raises(RuntimeError, match="overlaps"):
+            G.take_rows(ids, [out], out=[out])
+        loss.backward()
+        # tensors without a version counter
+        with torch.inference_mode():
+            acc, out = torch.zeros(5, device=DEV), torch.zeros(5, 3, device=DEV)
+            G.accumulate_weights(acc, torch.ones(5, device=DEV))
+            G.take_rows(ids, [torch.ones(9, 3, device=DEV)], out=[out])
+        assert (acc == 1).all() and (out == 1).all()
