@@ -399,8 +399,18 @@ def _keep_groups(what, P, budgets, groups, recent):
     """[(begin, end, keep, recent)] with keep and recent cut to what the group holds."""
     if groups is None:
         groups = [(0, P)]
-    groups = [(int(a), int(b)) for a, b in groups]
-    each = lambda v: [int(x) for x in v] if isinstance(v, (list, tuple)) else [int(v)] * len(groups)  # noqa: E731
+
+    def whole(v):  # (int() alone would make 0 of a share of the rows)
+        try:
+            n = int(v)
+        except (TypeError, ValueError, OverflowError):
+            n = None
+        if n is None or n != v:
+            raise RuntimeError(f"{what}: budgets, recent and groups must be whole numbers (got {v!r})")
+        return n
+
+    groups = [(whole(a), whole(b)) for a, b in groups]
+    each = lambda v: [whole(x) for x in v] if isinstance(v, (list, tuple)) else [whole(v)] * len(groups)  # noqa: E731
     budgets, recent = each(budgets), each(recent)
     if len(budgets) != len(groups) or len(recent) != len(groups):
         raise RuntimeError(f"{what}: one budget (and one recent) for each of the {len(groups)} groups, or one for all")
@@ -422,7 +432,7 @@ def keep_heaviest(weights, budgets, groups=None, recent=0):
 
     weights: float32 of P values (accumulated blend weights); groups: (begin, end) row
     ranges in ascending order, as merge_ply returns them (default: one group of all rows);
-    budgets and recent: a number for all groups or a list with one for each.  A group of n
+    budgets and recent: a whole number for all groups or a list with one for each.  A group of n
     rows keeps min(budget, n): its last `recent` ones and the heaviest of the others, of
     equals the lowest row; NaN counts as lighter than everything.  Rows in no group go."""
     _typed("keep_heaviest", weights=weights)

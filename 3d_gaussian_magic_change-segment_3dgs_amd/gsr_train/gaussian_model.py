@@ -410,7 +410,7 @@ class GaussianModel:
     @torch.no_grad()
     def evict(self, budget, recent=0, groups=None):
         """Bring the model -- or, with groups = [(begin, end)] as merge_ply returns them, each of
-        its scenes -- to at most `budget` Gaussians (a number, or a list with one for each
+        its scenes -- to at most `budget` Gaussians (a whole number, or a list with one for each
         group): the last `recent` ones (new Gaussians are appended) and the heaviest of the others by
         `contribution` stay, in order, with their moments and statistics; Gaussians in no group
         go.  The host does not wait for the device.  Returns (ids, groups): the old index of each

@@ -31,3 +31,15 @@ def test_sizes_that_do_not_fit_an_int_are_refused(route):
         refused(rows.dequantize, match="2\\^20")
     refused(G.mx4_quantize, meta(3, 2 ** 20), match="GPU")  # the widest
     refused(G.mx4_quantize, meta(0, 2 ** 21), match="GPU")  # nothing of any width
+
+
+def test_budgets_are_whole_numbers(route):
+    """A share of the rows is no budget: it would be cut to 0, and everything would go."""
+    import gsr_train as G
+    from gsr_train.compact import _keep_groups
+    w = torch.zeros(10)
+    for bad in (0.7, 2.5, [3, 0.5], float("nan"), float("inf"), torch.tensor(0.5), None, "5"):
+        refused(G.keep_heaviest, w, bad, [(0, 4), (4, 10)], match="whole numbers")
+        refused(G.keep_heaviest, w, 1, [(0, 4), (4, 10)], recent=bad, match="whole numbers")
+    refused(G.keep_heaviest, w, 1, [(0, 4.5)], match="whole numbers")
+    assert _keep_groups("x", 10, 1e1, [(0, 6.0), (torch.tensor(6), 10)], torch.tensor(2)) == [(0, 6, 6, 2), (6, 10, 4, 2)]
