@@ -1177,6 +1177,20 @@ unsigned grid_for(long long items, long long cap) {
 // One thread per Gaussian, its index an int: the last block's must not pass 2^31.
 constexpr int MAX_P = 0x7FFFFFFF - CP_THREADS;
 
+// Does a weight lie in the memory of a sum that is not its own?  (That sum is written before it is read, or after.)
+bool shared_apart(int P, const float* weights, long long stride, const float* acc) {
+    if (weights == acc && (stride == 1 || P == 1)) return false;
+    typedef __int128 wide;  // addresses in bytes: no product leaves it
+    wide step = 4 * (wide)stride, w = (wide)(uintptr_t)weights;
+    const wide a = (wide)(uintptr_t)acc, end = a + 4 * (wide)P;
+    if (step < 0) {  // from the other end
+        w += step * (P - 1);
+        step = -step;
+    }
+    const wide i = w + 4 > a ? 0 : step > 0 ? (a - w - 4) / step + 1 : P;  // the first weight that ends behind acc
+    return i < P && w + i * step < end;
+}
+
 int check_rows(long long R, int K) {
     if (R < 0 || K < 0 || K > GSR_MAX_WIDTH || (K > 0 && R > (1LL << 42) / K))  // (products of the two stay far from 2^63)
         return set_error("[gsr] mx4: invalid number or width of rows");
@@ -1319,6 +1333,8 @@ GSR_API int gsr_accumulate_weights(int P, const float* weights, long long stride
     if (P < 0 || P > MAX_P) return set_error("[gsr] gsr_accumulate_weights: invalid P");
     if (P == 0) return 0;
     if (!weights || !acc) return set_error("[gsr] gsr_accumulate_weights: null buffer");
+    if (shared_apart(P, weights, stride, acc))
+        return set_error("[gsr] gsr_accumulate_weights: the weights overlap the sums, element on another element");
     k_accumulate_weights<<<grid_for(P, 1LL << 31), CP_THREADS, 0, (hipStream_t)stream>>>(P, weights, stride, decay, acc);
     return launched("accumulate_weights");
 }

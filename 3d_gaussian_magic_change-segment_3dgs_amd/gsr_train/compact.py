@@ -380,7 +380,8 @@ def sh_colors_quantized(xyz, features, campos, degree):
 @torch.no_grad()
 def accumulate_weights(acc, weights, decay=1.0):
     """acc <- decay * acc + weights, in place: acc float32 contiguous of P values, weights
-    float32 [P] of any stride (a column of a [P, 3] gradient)."""
+    float32 [P] of any stride (a column of a [P, 3] gradient), which may be acc itself but not
+    overlap it otherwise."""
     _trace_check("accumulate_weights")
     _typed("accumulate_weights", acc=acc, weights=weights)
     P = acc.numel()

@@ -64,7 +64,8 @@ GSR_API int gsr_sh_colors_backward(int P, int V, int degree, int M, const float*
                                    const uint8_t* scales, const float* campos, const uint8_t* mask,
                                    const float* dcolors, float* dxyz, float* ddc, float* dfeatures, void* stream);
 
-/* acc[i] <- decay * acc[i] + weights[i * stride], i < P (accumulated blend weights). */
+/* acc[i] <- decay * acc[i] + weights[i * stride], i < P (accumulated blend weights).  The weights
+ * may be acc itself; weights that lie on another element's sum are refused. */
 GSR_API int gsr_accumulate_weights(int P, const float* weights, long long stride, float decay, float* acc,
                                    void* stream);
 

@@ -43,3 +43,16 @@ def test_budgets_are_whole_numbers(route):
         refused(G.keep_heaviest, w, 1, [(0, 4), (4, 10)], recent=bad, match="whole numbers")
     refused(G.keep_heaviest, w, 1, [(0, 4.5)], match="whole numbers")
     assert _keep_groups("x", 10, 1e1, [(0, 6.0), (torch.tensor(6), 10)], torch.tensor(2)) == [(0, 6, 6, 2), (6, 10, 4, 2)]
+
+
+def test_accumulated_weights_that_overlap_their_sum_are_refused():
+    """acc and weights in the same memory: only element on element (acc <- (decay + 1) acc) has one result."""
+    from gsr_train import compact as T
+    L = T._lib
+    call = lambda P, w, stride, acc: (L.gsr_accumulate_weights(P, w, stride, 1.0, acc, None),  # noqa: E731
+                                      L.gsr_last_error().decode())
+    a = 1 << 20
+    for P, w, stride in ((10, a + 4, 1), (10, a - 4, 1), (10, a - 36, 1), (10, a + 36, 1), (10, a, 2), (10, a - 8, 4),
+                         (10, a, 0), (10, a + 16, 0), (10, a - 36, 3), (2, a - 4, 1), (10, a + 36, -1), (10, a + 76, -2)):
+        rc, err = call(P, w, stride, a)
+        assert rc != 0 and "overlap" in err, (P, w - a, stride)

@@ -194,3 +194,26 @@ def test_writes_in_place_are_seen_by_autograd(monkeypatch):
             G.accumulate_weights(acc, torch.ones(5, device=DEV))
             G.take_rows(ids, [torch.ones(9, 3, device=DEV)], out=[out])
         assert (acc == 1).all() and (out == 1).all()
+
+
+def test_weights_beside_and_between_their_sums():
+    """acc in the middle of the memory that the weights are a strided view of: allowed where they share no element or
+    every element, each result that of separate tensors."""
+    import gsr_train as G
+    for P, start, stride in ((10, 50, 1), (1, 50, 5), (10, 60, 1), (10, 40, 1), (10, 49, 11), (10, 49, 0), (10, 60, 0),
+                             (5, 48, 30), (10, 10, 4), (4, 44, 10)):
+        buf = torch.rand(400, generator=gen(P * stride + start)).to(DEV)
+        acc, w = buf[50:50 + P], buf.as_strided((P,), (stride,), start)
+        want = acc.clone()
+        G.accumulate_weights(want, w.clone(), 0.5)
+        before = buf.clone()
+        G.accumulate_weights(acc, w, 0.5)
+        assert torch.equal(acc, want), (P, start, stride)
+        before[50:50 + P] = want
+        assert torch.equal(buf, before)
+    for P, start, stride in ((10, 51, 1), (10, 49, 1), (10, 50, 2), (10, 40, 5), (10, 55, 0)):
+        buf = torch.rand(400, generator=gen(1)).to(DEV)
+        before = buf.clone()
+        with pytest.raises(RuntimeError, match="overlap"):
+            G.accumulate_weights(buf[50:50 + P], buf.as_strided((P,), (stride,), start), 0.5)
+        assert torch.equal(buf, before)
