@@ -1183,12 +1183,15 @@ bool shared_apart(int P, const float* weights, long long stride, const float* ac
     typedef __int128 wide;  // addresses in bytes: no product leaves it
     wide step = 4 * (wide)stride, w = (wide)(uintptr_t)weights;
     const wide a = (wide)(uintptr_t)acc, end = a + 4 * (wide)P;
-    if (step < 0) {  // from the other end
+    const bool back = step < 0;
+    if (back) {  // from the other end
         w += step * (P - 1);
         step = -step;
     }
     const wide i = w + 4 > a ? 0 : step > 0 ? (a - w - 4) / step + 1 : P;  // the first weight that ends behind acc
-    return i < P && w + i * step < end;
+    if (i >= P || w + i * step >= end) return false;
+    const bool only = i + 1 == P || w + (i + 1) * step >= end;
+    return !only || w + i * step != a + 4 * (back ? P - 1 - i : i);
 }
 
 int check_rows(long long R, int K) {

@@ -198,10 +198,11 @@ def test_writes_in_place_are_seen_by_autograd(monkeypatch):
 
 def test_weights_beside_and_between_their_sums():
     """acc in the middle of the memory that the weights are a strided view of: allowed where they share no element or
-    every element, each result that of separate tensors."""
+    none but an element's own, each result that of separate tensors."""
     import gsr_train as G
     for P, start, stride in ((10, 50, 1), (1, 50, 5), (10, 60, 1), (10, 40, 1), (10, 49, 11), (10, 49, 0), (10, 60, 0),
-                             (5, 48, 30), (10, 10, 4), (4, 44, 10)):
+                             (5, 48, 30), (10, 10, 4), (4, 44, 10),
+                             (7, 30, 6)):
         buf = torch.rand(400, generator=gen(P * stride + start)).to(DEV)
         acc, w = buf[50:50 + P], buf.as_strided((P,), (stride,), start)
         want = acc.clone()
