@@ -1174,6 +1174,9 @@ unsigned grid_for(long long items, long long cap) {
     return (unsigned)(g < 1 ? 1 : g > cap ? cap : g);
 }
 
+// A launch has fewer than 2^32 threads.
+constexpr long long MAX_BLOCKS = ((1LL << 32) - 1) / CP_THREADS;
+
 // One thread per Gaussian, its index an int: the last block's must not pass 2^31.
 constexpr int MAX_P = 0x7FFFFFFF - CP_THREADS;
 
@@ -1231,7 +1234,7 @@ GSR_API int gsr_mx4_quantize(long long R, int K, const float* x, long long row_s
     if (row_stride < K && R > 1) return set_error("[gsr] gsr_mx4_quantize: rows overlap");
     const Tiling t = tiling(mx_blocks(K), MXQ_SPAN);
     const long long blocks = tiling_blocks(t, R, MXQ_SPAN);
-    if (blocks >= (1LL << 31)) return set_error("[gsr] gsr_mx4_quantize: too many rows in one call");
+    if (blocks > MAX_BLOCKS) return set_error("[gsr] gsr_mx4_quantize: too many rows in one call");
     k_mx4_quantize<<<(unsigned)blocks, CP_THREADS, 0, (hipStream_t)stream>>>(R, K, t, x, row_stride, codes, scales);
     return launched("mx4_quantize");
 }
@@ -1243,14 +1246,14 @@ GSR_API int gsr_mx4_dequantize(long long R, int K, const uint32_t* codes, const 
     if (!x || !codes || !scales) return set_error("[gsr] gsr_mx4_dequantize: null buffer");
     if (mxd_flat(K)) {
         const long long blocks = (R * K + MXD_SPAN - 1) / MXD_SPAN;
-        if (blocks >= (1LL << 31)) return set_error("[gsr] gsr_mx4_dequantize: too many rows in one call");
+        if (blocks > MAX_BLOCKS) return set_error("[gsr] gsr_mx4_dequantize: too many rows in one call");
         k_mx4_dequantize_flat<<<(unsigned)blocks, CP_THREADS, 0, (hipStream_t)stream>>>(
             R, K, (uint32_t)((1ULL << 32) / K + 1), codes, scales, x);
         return launched("mx4_dequantize");
     }
     const Tiling t = tiling((K + 3) / 4, CP_THREADS);
     const long long blocks = tiling_blocks(t, R, CP_THREADS);
-    if (blocks >= (1LL << 31)) return set_error("[gsr] gsr_mx4_dequantize: too many rows in one call");
+    if (blocks > MAX_BLOCKS) return set_error("[gsr] gsr_mx4_dequantize: too many rows in one call");
     k_mx4_dequantize<<<(unsigned)blocks, CP_THREADS, 0, (hipStream_t)stream>>>(
         R, K, t, reinterpret_cast<const uint16_t*>(codes), scales, x);
     return launched("mx4_dequantize");
@@ -1425,10 +1428,8 @@ GSR_API int gsr_take_rows(int K, const int* ids, int n, const gsr_rows* tensors,
         }
         if (clash) return set_error("[gsr] gsr_take_rows: a destination overlaps the ids or another tensor of the call");
     }
-    hipStream_t st = (hipStream_t)stream;
-    bool any = false;
-    for (int k0 = 0; k0 < n; k0 += TAKE_MAX) {
-        TakeArgs a{};
+    // the tensors of a launch: their blocks, or -1 where a launch does not hold them
+    auto launch_of = [&](int k0, TakeArgs& a) -> long long {
         long long blocks = 0;
         for (int k = k0; k < n && k < k0 + TAKE_MAX; ++k) {
             const gsr_rows& q = tensors[k];
@@ -1440,7 +1441,24 @@ GSR_API int gsr_take_rows(int K, const int* ids, int n, const gsr_rows* tensors,
             const long long nb = std::max(1LL, tiling_blocks(t, rows, TAKE_SPAN));
             a.t[a.n++] = {q.src, q.dst, t, rows, q.rows, unit, q.pad, (uint32_t)blocks, (uint32_t)nb};
             blocks += nb;
-            if (blocks >= (1LL << 31)) return set_error("[gsr] gsr_take_rows: too many rows in one call");
+            if (blocks > MAX_BLOCKS) return -1;
+        }
+        return blocks;
+    };
+    hipStream_t st = (hipStream_t)stream;
+    TakeArgs a{};
+    long long blocks = launch_of(0, a);
+    bool fits = blocks >= 0;
+    for (int k0 = TAKE_MAX; k0 < n && fits; k0 += TAKE_MAX) {  // (before the first launch)
+        TakeArgs later{};
+        fits = launch_of(k0, later) >= 0;
+    }
+    if (!fits) return set_error("[gsr] gsr_take_rows: too many rows in one call");
+    bool any = false;
+    for (int k0 = 0; k0 < n; k0 += TAKE_MAX) {
+        if (k0 > 0) {
+            a = TakeArgs{};
+            blocks = launch_of(k0, a);
         }
         if (a.n == 0) continue;
         any = true;

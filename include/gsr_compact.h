@@ -30,6 +30,9 @@ extern "C" {
 #define GSR_MX_BLOCK 32
 #define GSR_MAX_WIDTH (1 << 20) /* words of a row, K or width below */
 
+/* A launch has fewer than 2^32 threads: calls that would need more are refused (decoding more than 17e9
+ * values, for one), before they write anything. */
+
 /* R rows of K floats, row i at x + i * row_stride -> codes, scales (codes 4-B aligned). */
 GSR_API int gsr_mx4_quantize(long long R, int K, const float* x, long long row_stride, uint32_t* codes,
                              uint8_t* scales, void* stream);

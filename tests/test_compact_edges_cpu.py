@@ -56,3 +56,16 @@ def test_accumulated_weights_that_overlap_their_sum_are_refused():
                          (10, a, 0), (10, a + 16, 0), (10, a - 36, 3), (2, a - 4, 1), (10, a + 36, -1), (10, a + 76, -2)):
         rc, err = call(P, w, stride, a)
         assert rc != 0 and "overlap" in err, (P, w - a, stride)
+
+
+def test_calls_larger_than_a_grid_are_refused_by_name():
+    """A launch has fewer than 2^32 threads: 2^24 - 1 blocks of 256."""
+    from gsr_train import compact as T
+    L = T._lib
+    err = lambda: L.gsr_last_error().decode()  # noqa: E731
+    most = 2 ** 24 - 1
+    for R, K in ((most * 1024 // 45 + 1, 45), (most * 1024 // 4 + 1, 4), (most * 256 + 1, 1), (most * 128 + 1, 34),
+                 (most + 1, 1024), (most // 2, 4096)):  # 1024 values a block, or 256 pieces of four
+        assert L.gsr_mx4_dequantize(R, K, 4096, 4096, 4096, None) != 0 and "too many rows in one call" in err(), (R, K)
+    for R, K in ((most * 128 + 1, 9), (most * 64 + 1, 45), (most + 1, 32 * 128), (most, 32 * 129)):  # 128 blocks of 32
+        assert L.gsr_mx4_quantize(R, K, 4096, K, 4096, 4096, None) != 0 and "too many rows in one call" in err(), (R, K)

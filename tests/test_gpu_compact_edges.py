@@ -218,3 +218,15 @@ def test_weights_beside_and_between_their_sums():
         with pytest.raises(RuntimeError, match="overlap"):
             G.accumulate_weights(buf[50:50 + P], buf.as_strided((P,), (stride,), start), 0.5)
         assert torch.equal(buf, before)
+
+
+def test_rows_moved_are_counted_before_the_first_launch():
+    """The 33rd tensor goes into a second launch; that it is too large is said before the first one writes."""
+    from gsr_train import compact as T
+    dst = torch.full((32, 4), 9.0, device=DEV)
+    small = [(dst.data_ptr(), dst[k].data_ptr(), 0, 0, 1) for k in range(32)]  # a word of padding each
+    large = (1 << 52, 1 << 55, 768 * 8, 5, 0)  # 2 or more blocks a row, of 2^31 - 1 rows
+    table = (T._Rows * 33)(*small, large)
+    with pytest.raises(RuntimeError, match="too many rows in one call"):
+        T._call(dst.device, T._lib.gsr_take_rows, 2 ** 31 - 1, 64, 33, table)
+    assert (dst == 9).all()
