@@ -69,3 +69,38 @@ def test_calls_larger_than_a_grid_are_refused_by_name():
         assert L.gsr_mx4_dequantize(R, K, 4096, 4096, 4096, None) != 0 and "too many rows in one call" in err(), (R, K)
     for R, K in ((most * 128 + 1, 9), (most * 64 + 1, 45), (most + 1, 32 * 128), (most, 32 * 129)):  # 128 blocks of 32
         assert L.gsr_mx4_quantize(R, K, 4096, K, 4096, 4096, None) != 0 and "too many rows in one call" in err(), (R, K)
+
+
+# ---- the counters of the benchmark line -----------------------------------------------------------
+def test_counters_stand_for_the_sources_of_the_kernels_they_describe(tmp_path, monkeypatch):
+    """The committed counter summary is the renderer's: it holds as long as the renderer's sources stay, whatever
+    other sources the library is linked from."""
+    import os
+    import shutil
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    monkeypatch.syspath_prepend(root)
+    monkeypatch.syspath_prepend(os.path.join(root, "tools"))
+    import bench
+    import pmc_summary
+    summary, note = bench.pmc_for_this_build()
+    assert summary is not None, note
+    bwd = summary["kernels"]["render_bwd"]
+    assert bwd["hbm_bytes_per_launch"] > 0 and bwd["SQ_INSTS_VALU"] > 0
+    pkg = "3d_gaussian_magic_change-segment_3dgs_amd"
+    shutil.copytree(os.path.join(root, pkg, "csrc"), tmp_path / pkg / "csrc")
+    shutil.copytree(os.path.join(root, "include"), tmp_path / "include")
+    monkeypatch.setattr(pmc_summary, "ROOT", str(tmp_path))
+    csrc = tmp_path / pkg / "csrc"
+    assert pmc_summary.sources_sha256() == summary["sources_sha256"]
+    (csrc / "compact.hip").write_text("// other kernels\n")
+    assert pmc_summary.sources_sha256() == summary["sources_sha256"]
+    for name in ("render_bwd.hip", "api.hip", "gsr_internal.h", "new.hip"):
+        old = (csrc / name).read_text() if (csrc / name).exists() else None
+        (csrc / name).write_text((old or "") + "\n")
+        assert pmc_summary.sources_sha256() != summary["sources_sha256"], name
+        if old is None:
+            (csrc / name).unlink()
+        else:
+            (csrc / name).write_text(old)
+    assert "pmc_summary" in sys.modules
