@@ -104,3 +104,14 @@ def test_counters_stand_for_the_sources_of_the_kernels_they_describe(tmp_path, m
         else:
             (csrc / name).write_text(old)
     assert "pmc_summary" in sys.modules
+
+
+def test_rows_of_codes_fit_every_width_of_their_words():
+    """24 bytes of codes and 2 scales are rows of 41 to 48 values."""
+    import gsr_train as G
+    codes, scales = torch.zeros(5, 24, dtype=torch.uint8), torch.zeros(5, 2, dtype=torch.uint8)
+    for width in range(41, 49):
+        assert G.MX4Rows(codes, scales, width).width == width
+    refused(G.MX4Rows, codes, scales, 40, match="codes")
+    refused(G.MX4Rows, codes, scales, 49, match="codes")
+    refused(G.MX4Rows, codes, scales[:, :1].contiguous(), 44, match="scales")

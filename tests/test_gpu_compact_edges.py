@@ -230,3 +230,45 @@ def test_rows_moved_are_counted_before_the_first_launch():
     with pytest.raises(RuntimeError, match="too many rows in one call"):
         T._call(dst.device, T._lib.gsr_take_rows, 2 ** 31 - 1, 64, 33, table)
     assert (dst == 9).all()
+
+
+# ---- values that the tests of the operators left out ----------------------------------------------
+@pytest.mark.parametrize("n,pieces", [(5_000_011, 2), (60_000_003, 15)])
+@pytest.mark.parametrize("kind", ["equal", "few", "heavy"])
+def test_keep_heaviest_of_tiles_of_several_pieces(n, pieces, kind):
+    """A block takes two pieces of a tile, and as many as 16-bit counts allow: 15 of 4096 rows, all of them equal."""
+    import gsr_train as G
+    assert min(15, max(1, (n // 4096 + 1023) // 1024)) == pieces
+    g = torch.Generator(device=DEV).manual_seed(n)
+    w = torch.rand(n, device=DEV, generator=g)
+    if kind == "equal":
+        w.fill_(0.5)
+    elif kind == "few":
+        w = (w * 3).floor()
+    else:
+        w = torch.exp(w * 40 - 20)
+    for budget, recent in ((n * 2 // 3, 0), (n // 5, 12_345), (n - 1, 0)):
+        old = n - recent
+        order = torch.sort(w[:old], descending=True, stable=True)[1][:budget - recent]
+        keep = torch.zeros(n, dtype=torch.bool, device=DEV)
+        keep[order] = True
+        keep[old:] = True
+        want = torch.nonzero(keep).flatten().int()
+        assert torch.equal(G.keep_heaviest(w, budget, recent=recent), want), budget
+
+
+@pytest.mark.parametrize("degree", [0, 3])
+def test_gradient_on_both_sides_of_zero(degree):
+    """The constants next to -1 / (2 C_0), at the camera, where the direction and all other terms are 0: p >= 0 takes
+    part.  (p = 0 itself is out of reach here: C_0 times a float is never -1/2.)"""
+    import gsr_train as G
+    C0 = 0.28209479177387814
+    dc = torch.tensor(-0.5 / C0, dtype=torch.float64).float()
+    f = torch.zeros(3, 16, 3)
+    f[0, 0], f[1, 0], f[2, 0] = dc, torch.nextafter(dc, torch.tensor(-9.0)), torch.nextafter(dc, torch.tensor(9.0))
+    p = 0.5 + C0 * f[:, 0].double()
+    assert (p.abs() < 2.0 ** -22).all() and (p > 0).any() and (p < 0).any()
+    fg = f.to(DEV).requires_grad_()
+    c = G.sh_colors_quantized(torch.zeros(3, 3, device=DEV), fg, torch.zeros(3, device=DEV), degree)
+    (gf,) = torch.autograd.grad(c, fg, torch.ones(3, 3, device=DEV))
+    assert torch.equal(gf[:, 0].cpu() != 0, p >= 0) and (gf[:, 1:] == 0).all()
