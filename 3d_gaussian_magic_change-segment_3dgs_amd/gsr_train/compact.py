@@ -21,6 +21,7 @@ captured backward pass would have to wait on the eager graph's stream.  torch.ji
 sh_colors and sh_colors_quantized as calls of them; the other operators, and all of them under
 make_fx, refuse to be traced."""
 import ctypes
+import numbers
 
 import torch
 from torch.fx.experimental.proxy_tensor import get_proxy_mode
@@ -310,7 +311,7 @@ class _ShColorsQuantized(torch.autograd.Function):
 def _plain(a, b, c, degree):
     """What the C++ binding takes; anything else is refused (or converted) below."""
     return isinstance(a, torch.Tensor) and isinstance(b, torch.Tensor) and isinstance(c, torch.Tensor) and \
-        type(degree) is int
+        (type(degree) is int or isinstance(degree, numbers.Integral))
 
 
 def sh_colors(xyz, features_dc, rest, campos, degree):

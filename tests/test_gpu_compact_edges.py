@@ -272,3 +272,25 @@ def test_gradient_on_both_sides_of_zero(degree):
     c = G.sh_colors_quantized(torch.zeros(3, 3, device=DEV), fg, torch.zeros(3, device=DEV), degree)
     (gf,) = torch.autograd.grad(c, fg, torch.ones(3, 3, device=DEV))
     assert torch.equal(gf[:, 0].cpu() != 0, p >= 0) and (gf[:, 1:] == 0).all()
+
+
+def test_degrees_of_other_integer_types_take_the_compiled_route(monkeypatch):
+    """numpy integers, as a loaded scene may hold them: no slower call, and capture with gradients works."""
+    import numpy as np
+    import gsr_train as G
+    from gsr_train import compact as T
+    xyz, f, cam, up = (t.to(DEV) for t in scene(30, 9, 1, 4))
+    rest = G.mx4_quantize(f.flatten(1)[:, 3:])
+    want, shown = G.sh_colors_quantized(xyz, f, cam, 2), G.sh_colors(xyz, f[:, 0], rest, cam, 2)
+    monkeypatch.setattr(T, "_sh_check", None)  # what the ctypes route begins with
+    for degree in (np.int64(2), np.int32(2), np.uint8(2)):
+        assert torch.equal(G.sh_colors_quantized(xyz, f, cam, degree), want)
+        assert torch.equal(G.sh_colors(xyz, f[:, 0], rest, cam, degree), shown)
+    x = xyz.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (g,) = torch.autograd.grad(G.sh_colors_quantized(x, f, cam, np.int64(2)), x, up)
+    graph.replay()
+    torch.cuda.synchronize()
+    (h,) = torch.autograd.grad(G.sh_colors_quantized(x, f, cam, 2), x, up)
+    assert torch.equal(g, h)
