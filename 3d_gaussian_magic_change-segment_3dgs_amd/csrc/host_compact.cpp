@@ -64,6 +64,11 @@ void check_traced(const char* what, bool traced = jit_traced() || fx_traced()) {
     if (traced) refuse(std::string(what) + ": cannot be traced");
 }
 
+// A write through the pointer, which autograd has to know of.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // (the library takes a width as an int)
 void check_width(const char* what, int64_t K) {
     if (K > GSR_MAX_WIDTH) refuse(std::string(what) + ": rows of more than 2^20 values");
@@ -352,6 +357,24 @@ at::Tensor sh_colors_quantized(const at::Tensor& xyz_, const at::Tensor& feature
     return quantized_of(xyz, features, campos, degree, single, held);
 }
 
+void accumulate_weights(const at::Tensor& acc, const at::Tensor& weights, double decay) {
+    const char* what = "accumulate_weights";
+    check_traced(what);
+    check_float(what, "acc", acc);
+    check_float(what, "weights", weights);
+    const int64_t P = acc.numel();
+    if (P >= (1LL << 31)) refuse("accumulate_weights: at most 2^31 - 1 weights");
+    if (!acc.is_contiguous() || weights.dim() != 1 || weights.size(0) != P)
+        refuse("accumulate_weights: acc must be contiguous and weights have shape (P,), P values each");
+    check_gpu(what, acc);
+    check_device(what, "weights", weights, acc);
+    Guard guard(acc.device());
+    if (!P) return;
+    check(gsr_accumulate_weights((int)P, weights.data_ptr<float>(), weights.stride(0), (float)decay,
+                                 acc.data_ptr<float>(), cur_stream()));
+    written(acc);
+}
+
 at::Tensor keep_heaviest(const at::Tensor& weights, const std::vector<std::tuple<int, int, int, int>>& plan) {
     check_traced("keep_heaviest");
     Guard guard(weights.device());
@@ -408,9 +431,8 @@ std::vector<at::Tensor> take_rows(const at::Tensor& ids, const std::vector<at::T
         table.push_back({t.data_ptr(), out[n].data_ptr(), (int)width, (int)t.size(0), pad.empty() ? 0 : pad[n]});
     }
     if (!table.empty()) check(gsr_take_rows((int)K, ids.data_ptr<int>(), (int)table.size(), table.data(), cur_stream()));
-    if (given)  // a write that autograd has to know of
-        for (const at::Tensor& o : out)
-            if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
+    if (given)
+        for (const at::Tensor& o : out) written(o);
     return out;
 }
 
@@ -420,6 +442,7 @@ void bind_compact(pybind11::module_& mod) {
     mod.def("mx4_dequantize", &mx4_dequantize, py::call_guard<py::gil_scoped_release>());
     mod.def("sh_colors", &sh_colors, py::call_guard<py::gil_scoped_release>());
     mod.def("sh_colors_quantized", &sh_colors_quantized, py::call_guard<py::gil_scoped_release>());
+    mod.def("accumulate_weights", &accumulate_weights, py::call_guard<py::gil_scoped_release>());
     mod.def("keep_heaviest", &keep_heaviest, py::call_guard<py::gil_scoped_release>());
     mod.def("take_rows", &take_rows, py::call_guard<py::gil_scoped_release>());
 }

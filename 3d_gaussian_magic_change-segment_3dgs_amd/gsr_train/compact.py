@@ -383,6 +383,8 @@ def accumulate_weights(acc, weights, decay=1.0):
     """acc <- decay * acc + weights, in place: acc float32 contiguous of P values, weights
     float32 [P] of any stride (a column of a [P, 3] gradient), which may be acc itself but not
     overlap it otherwise."""
+    if _HOST is not None and isinstance(acc, torch.Tensor) and isinstance(weights, torch.Tensor):
+        return _HOST.accumulate_weights(acc, weights, float(decay))
     _trace_check("accumulate_weights")
     _typed("accumulate_weights", acc=acc, weights=weights)
     P = acc.numel()
@@ -397,22 +399,24 @@ def accumulate_weights(acc, weights, decay=1.0):
         _written(acc)
 
 
+def _whole(what, v):
+    """v as an int (which int() alone would make of a share of the rows too: 0)."""
+    if type(v) is int:
+        return v
+    try:
+        n = int(v)
+    except (TypeError, ValueError, OverflowError):
+        n = None
+    if n is None or n != v:
+        raise RuntimeError(f"{what}: budgets, recent and groups must be whole numbers (got {v!r})")
+    return n
+
+
 def _keep_groups(what, P, budgets, groups, recent):
     """[(begin, end, keep, recent)] with keep and recent cut to what the group holds."""
-    if groups is None:
-        groups = [(0, P)]
-
-    def whole(v):  # (int() alone would make 0 of a share of the rows)
-        try:
-            n = int(v)
-        except (TypeError, ValueError, OverflowError):
-            n = None
-        if n is None or n != v:
-            raise RuntimeError(f"{what}: budgets, recent and groups must be whole numbers (got {v!r})")
-        return n
-
-    groups = [(whole(a), whole(b)) for a, b in groups]
-    each = lambda v: [whole(x) for x in v] if isinstance(v, (list, tuple)) else [whole(v)] * len(groups)  # noqa: E731
+    groups = [(0, P)] if groups is None else [(_whole(what, a), _whole(what, b)) for a, b in groups]
+    each = lambda v: [_whole(what, x) for x in v] if isinstance(v, (list, tuple)) else \
+        [_whole(what, v)] * len(groups)  # noqa: E731
     budgets, recent = each(budgets), each(recent)
     if len(budgets) != len(groups) or len(recent) != len(groups):
         raise RuntimeError(f"{what}: one budget (and one recent) for each of the {len(groups)} groups, or one for all")
@@ -446,12 +450,12 @@ def keep_heaviest(weights, budgets, groups=None, recent=0):
 
 def _keep(weights, plan):
     """keep_heaviest of a finished plan (_keep_groups)."""
-    _trace_check("keep_heaviest")
     P = weights.numel()
     _on_gpu("keep_heaviest", weights)
     weights = weights.contiguous()
     if _HOST is not None:
         return _HOST.keep_heaviest(weights, plan)
+    _trace_check("keep_heaviest")
     ids = torch.empty(sum(k for _, _, k, _ in plan), dtype=torch.int32, device=weights.device)
     if ids.numel():
         ws = torch.empty(int(_lib.gsr_keep_ws_bytes(P)), dtype=torch.uint8, device=weights.device)
