@@ -453,10 +453,12 @@ __device__ __forceinline__ void write_colors(const ShArgs& a, int i, v3a p, Coef
     }
 }
 
-// Colours that do not fit the caches beside the inputs pass by them (write-back of their lines
-// stands in the way of reads, the next kernel's too): 28.8 MB (300k Gaussians, 8 views) 10.7 -> 9.3 us, 72 MB (6M,
-// one view) 65.7 -> 62.6, 48 MB in a training step of 1M with 4 views 111 -> 96; 12 MB (1M, one view) 10.5 -> 10.6.
-// (The same for reading their gradients: backward 48 -> 62 us, so not there.)
+// Colours from 16 MB on, a sixteenth of the 256 MB cache, pass by the caches: write-back of their lines stands in the way of
+// reads.  Both sides, through and past, with inputs that change from pass to pass and with the same ones again: 8 views of 300k
+// Gaussians (28.8 MB) 13.4 and 10.3, 12.0 and 9.2 us; of 175k (16.8 MB) 8.3 and 7.2, 8.3 and 7.0; of 130k (12.5 MB) 7.1 and 6.1,
+// 6.5 and 5.9; one view of 4M (48 MB) 44.0 and 41.4, 34.4 and 34.5; of 1M (12 MB) 13.3 and 12.5, 10.9 and 11.4.  From 16 MB on
+// the kernel is as fast or faster past them, while the next reader of the colours pays 5 to 25 % for it (a pass right behind 8
+// views of 250k: both together 20.2 and 21.1, 22.0 and 20.8; behind 1M 19.7 and 19.5, 16.2 and 17.0).
 constexpr long long NT_COLOR_BYTES = 16LL << 20;
 
 // One thread per Gaussian, its coefficients in registers for all views.  Bound by memory with
@@ -481,11 +483,14 @@ constexpr int ROW16 = 13;                  // float4s
 constexpr int ROWS_LDS = 64 * 4 * ROW16;   // floats a wave (also 64 rows of 45)
 __device__ __forceinline__ void wave_lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// With NT the rows pass by the caches: what those hold of a tensor that does not fit them is gone
-// before its next reader comes, and was in the way of other data until then.  Loads of 192 MB of
-// features (1M Gaussians, one view): forward 43 -> 40 us, a step 86 -> 78; of 115 MB (600k, 8 views) a step 99 -> 86;
-// of 58 MB (300k): forward 14.0 -> 15.2, so not there.
-// Stores of the gradient: 192 MB, backward 49 -> 39 us; 58 MB and 8 views, 31 -> 24.
+// With NT rows of 48 floats pass by the caches (the others, F != 48, go through them whatever NT says).  Both sides,
+// through and past, one view.  Loads (forward), inputs that change: 58 MB of features (300k Gaussians) 18.8 and 15.3 us, 115 MB 32.5 and
+// 28.6, 192 MB 62.0 and 45.6; the same inputs again: 58 MB 13.3 and 14.6, 96 MB 19.5 and 21.7, 154 MB 43.9 and 32.6, as the
+// pass no longer fits the 256 MB cache.  In training every step goes through parameters, gradients and two moments, five
+// times the features: from 52 MB of features on that is more than the cache holds, and the first case is the nearer one.
+// Stores (the gradient): 29 MB 8.2 and 7.7, 8.5 and 7.7 with the same inputs; 58 MB 15.8 and 14.0, 13.5 and 12.9; 192 MB 45.1
+// and 42.7, 45.3 and 40.9.  No crossing here either; a reader right behind pays 17 % at 58 MB, forward,
+// backward and reader together 53.0 and 54.6, at 19 MB 23.5 and 23.6.  32 MB: an eighth of the cache.
 constexpr long long NT_LOAD_BYTES = 64LL << 20, NT_STORE_BYTES = 32LL << 20;
 template <bool NT>
 __device__ __forceinline__ void rows_in(const float* __restrict__ src, int rows, int F, float* lds, int lane) {
@@ -686,7 +691,8 @@ __global__ void __launch_bounds__(CP_THREADS) k_sh_colors_backward(ShArgs a, con
     }
 }
 
-// Bound by memory, 12 bytes a row; one thread each (a strided column of a gradient has nothing wide to load).
+// Bound by memory: 12 bytes a row, or the 20 that a column of a [P, 3] gradient fetches (what its caller has); one thread
+// each (a column has nothing wide to load).  1M rows 3.8 us, of a column 4.7.
 __global__ void __launch_bounds__(CP_THREADS) k_accumulate_weights(int P, const float* __restrict__ w,
                                                                    long long stride, float decay,
                                                                    float* __restrict__ acc) {
@@ -821,7 +827,7 @@ __device__ __forceinline__ bool keep_flat(const uint32_t (&key)[N], bool all_in)
     return x == 0 && all_in;
 }
 
-// Keys [i, i + N) of rows below `end` (0 behind it).
+// Keys [i, i + N) of rows below `end` (behind it that of 0.0: every reader goes by the row).
 template <int N>
 __device__ __forceinline__ void keep_load(const float* __restrict__ w, long long i, long long end, uint32_t (&key)[N]) {
     v4a v[N / 4];
@@ -1075,8 +1081,8 @@ __global__ void __launch_bounds__(CP_THREADS) k_keep_write(KeepArgs a, KeepWs ws
 // TAKE_SPAN units of one tensor's output, a unit being 16 bytes where the rows are whole and aligned
 // float4s (the features, 48 of a Gaussian's 61 floats, and the rotations), else the largest of 12, 8 and
 // 4 that a row is made of (with 4 for all of those, their blocks were 40 % of the launch for 15 % of the
-// bytes).  Loads and stores of 16 and 12 bytes pass by the caches: every line is wanted by one
-// instruction.  1M rows of 732 bytes kept at 70 %: 181 us, 5.7 TB/s of what has to move; with units of 16
+// bytes).  All loads, and the stores of 16 and 12 bytes, pass by the caches: a line is wanted by
+// one instruction.  1M rows of 732 bytes kept at 70 %: 181 us, 5.7 TB/s of what has to move; with units of 16
 // and 4 bytes only 196, with temporal accesses 215.  Narrow rows cost the lines of their dropped neighbours too.
 constexpr int TAKE_MAX = 32;    // tensors a launch
 // Units a thread: their ids, then their values, are in flight together.  3: a block is 64 rows of 192 bytes,

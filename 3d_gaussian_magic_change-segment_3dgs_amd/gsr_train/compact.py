@@ -2,7 +2,7 @@
 csrc/compact.hip).
 
 * `mx4_quantize` / `MX4Rows`: rows of floats -- the SH coefficients above the constant
-  one, 180 of a Gaussian's 236 bytes -- in 4-bit microscaled floating point (26 bytes).
+  one, 180 of a Gaussian's 244 bytes -- in 4-bit microscaled floating point (26 bytes).
 * `sh_colors`: view-dependent colours straight from the codes, with gradients for the
   positions and the constant coefficients; `sh_colors_quantized`: the same from the fp32
   features, which are rounded to 4 bits in the call and get their gradient straight
@@ -533,7 +533,7 @@ def take_gaussians(spec, ids, arenas):
 # ---- a trained scene for rendering --------------------------------------------------------------
 class CompactGaussians:
     """A GaussianModel as it is rendered after training, with the SH coefficients above the
-    constant one in 4 bits: 92 bytes a Gaussian at degree 3 and two classes where the model's arena and
+    constant one in 4 bits: 90 bytes a Gaussian at degree 3 and two classes where the model's arena and
     activations take 284 (and its moments twice 244 more).  Made by GaussianModel.compact();
     offers what render() reads (get_xyz, get_colors, get_opacity, get_scaling,
     get_rotation, get_segment, get_features), all without gradients."""
