@@ -458,7 +458,8 @@ __device__ __forceinline__ void write_colors(const ShArgs& a, int i, v3a p, Coef
 // Gaussians (28.8 MB) 13.4 and 10.3, 12.0 and 9.2 us; of 175k (16.8 MB) 8.3 and 7.2, 8.3 and 7.0; of 130k (12.5 MB) 7.1 and 6.1,
 // 6.5 and 5.9; one view of 4M (48 MB) 44.0 and 41.4, 34.4 and 34.5; of 1M (12 MB) 13.3 and 12.5, 10.9 and 11.4.  From 16 MB on
 // the kernel is as fast or faster past them, while the next reader of the colours pays 5 to 25 % for it (a pass right behind 8
-// views of 250k: both together 20.2 and 21.1, 22.0 and 20.8; behind 1M 19.7 and 19.5, 16.2 and 17.0).
+// views of 250k: both together 20.2 and 21.1, 22.0 and 20.8; behind 1M 19.7 and 19.5, 16.2 and 17.0).  Their gradients are read
+// through the caches at any size (past them, backward of 1M with 4 views 48 -> 62 us).
 constexpr long long NT_COLOR_BYTES = 16LL << 20;
 
 // One thread per Gaussian, its coefficients in registers for all views.  Bound by memory with
